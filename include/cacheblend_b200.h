@@ -430,6 +430,72 @@ CB_API int cb_sparse_q_scores_static(const void* query, int64_t query_token_stri
                                      float scale, float* scores, int32_t* device_error,
                                      void* stream);
 
+/*
+ * Fresh keys and values into the paged cache, K (and the queries, if any)
+ * rotated at their positions on the way.  key, value: [num_tokens]
+ * [num_kv_heads][head_size] with token and head strides; query (nullable, then
+ * num_q_heads 0) and query_out alike, not overlapping.  cos_sin:
+ * [max_position][rotary_dim] fp32 or of type `dtype` (cos half, then sin half);
+ * rotary_dim 0 copies K as it is (positions and cos_sin may be NULL).  The
+ * products and their sum are rounded to fp32 each, the result once to `dtype`.
+ * Token t goes to slot slots[t] of the paged planes; a negative slot is padding
+ * and nothing is written for it, nor for a slot outside the cache or a position
+ * outside the table (such a query row is zeros).  The slots of a call must be
+ * distinct, and the inputs must not overlap the pages.  No counterpart in
+ * cacheblend_vllm (vLLM's rotary module and cache write).
+ */
+CB_API int cb_append_paged_kv(const void* key, int64_t key_token_stride, int64_t key_head_stride,
+                              const void* value, int64_t value_token_stride,
+                              int64_t value_head_stride, const void* query,
+                              int64_t query_token_stride, int64_t query_head_stride, void* query_out,
+                              int64_t query_out_token_stride, int64_t query_out_head_stride,
+                              int64_t num_tokens, int64_t num_q_heads, int64_t num_kv_heads,
+                              int64_t head_size, int dtype, const int64_t* positions,
+                              const void* cos_sin, int cos_sin_dtype, int64_t max_position,
+                              int64_t rotary_dim, int is_neox, void* k_cache, void* v_cache,
+                              int64_t block_stride, int64_t slot_stride, int64_t head_stride,
+                              int64_t num_blocks, int64_t block_size, const int64_t* slots,
+                              void* stream);
+
+/*
+ * The same into 4-bit pages.  A row of head_size (64 or 128) values is
+ * head_size / 2 bytes of codes (dimension 2i in the low nibble of byte i) and,
+ * per group of 64 values, a pair of fp16: step and lowest value; a value is
+ * lowest + step * code.  The row is rounded to `dtype` first; lowest =
+ * fp16(min), step = fp16((max - min) / 15), codes to the nearest.  Values beyond
+ * +-65504 are held there, a group with a NaN or an infinity gets a NaN step.
+ * Codes and scales have strides of their own (block, row, head; bytes); codes
+ * rows are 16-byte aligned, the pairs of a row head_size / 16 bytes.
+ */
+CB_API int cb_append_paged_kv4(const void* key, int64_t key_token_stride, int64_t key_head_stride,
+                               const void* value, int64_t value_token_stride,
+                               int64_t value_head_stride, const void* query,
+                               int64_t query_token_stride, int64_t query_head_stride,
+                               void* query_out, int64_t query_out_token_stride,
+                               int64_t query_out_head_stride, int64_t num_tokens,
+                               int64_t num_q_heads, int64_t num_kv_heads, int64_t head_size,
+                               int dtype, const int64_t* positions, const void* cos_sin,
+                               int cos_sin_dtype, int64_t max_position, int64_t rotary_dim,
+                               int is_neox, void* k_codes, void* v_codes, int64_t block_stride,
+                               int64_t slot_stride, int64_t head_stride, void* k_scales,
+                               void* v_scales, int64_t scale_block_stride,
+                               int64_t scale_slot_stride, int64_t scale_head_stride,
+                               int64_t num_blocks, int64_t block_size, const int64_t* slots,
+                               void* stream);
+
+/*
+ * Rows of 4-bit pages as values: out[plane, t] = the row of slots[t], rounded
+ * once to `dtype`; zeros for a slot outside the cache (padding).
+ */
+CB_API int cb_gather_paged_kv4(const void* k_codes, const void* v_codes, int64_t block_stride,
+                               int64_t slot_stride, int64_t head_stride, const void* k_scales,
+                               const void* v_scales, int64_t scale_block_stride,
+                               int64_t scale_slot_stride, int64_t scale_head_stride,
+                               int64_t num_blocks, int64_t block_size, int64_t num_heads,
+                               int64_t head_size, const int64_t* slots, int64_t num_tokens,
+                               void* out, int64_t out_plane_stride, int64_t out_token_stride,
+                               int64_t out_head_stride, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,6 +7,7 @@ mirrors of the reference types: ``CacheBlendConfig``, ``BlendPlan``,
 ``LocalPinnedCPUStore``, ``PipelineTracer``.
 """
 
+from .append import PagedKV4, append_paged_kv, append_paged_kv4, gather_paged_kv4
 from .config import CacheBlendConfig
 from .kv_layout import gather_paged_kv, scatter_paged_kv
 from .loader import PagedBlendLoader
@@ -22,9 +23,13 @@ __all__ = [
     "CacheBlendConfig",
     "LocalPinnedCPUStore",
     "PagedBlendLoader",
+    "PagedKV4",
     "PipelineTracer",
     "SegmentId",
+    "append_paged_kv",
+    "append_paged_kv4",
     "gather_paged_kv",
+    "gather_paged_kv4",
     "kv_deviation",
     "recompute_budget",
     "relocate_key",

@@ -21,7 +21,7 @@ LIB_PATH = Path(
     os.environ.get("CACHEBLEND_B200_LIB")
     or Path(__file__).resolve().parent / "_lib" / "libcacheblend_b200.so"
 )
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 CB_OK = 0
 CB_ERR_INVALID = -1
@@ -133,6 +133,23 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _i32,
         [_ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _i64, _i32, _ptr, _ptr, _i64,
          ctypes.c_float, _ptr, _ptr, _ptr],
+    ),
+    "cb_append_paged_kv": (
+        _i32,
+        [_ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _i64,
+         _i64, _i32, _ptr, _ptr, _i32, _i64, _i64, _i32, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64,
+         _ptr, _ptr],
+    ),
+    "cb_append_paged_kv4": (
+        _i32,
+        [_ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _i64,
+         _i64, _i32, _ptr, _ptr, _i32, _i64, _i64, _i32, _ptr, _ptr, _i64, _i64, _i64, _ptr, _ptr,
+         _i64, _i64, _i64, _i64, _i64, _ptr, _ptr],
+    ),
+    "cb_gather_paged_kv4": (
+        _i32,
+        [_ptr, _ptr, _i64, _i64, _i64, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _ptr,
+         _i64, _ptr, _i64, _i64, _i64, _i32, _ptr],
     ),
 }
 
