@@ -14,6 +14,7 @@ CUDA tensors only.
 
 from __future__ import annotations
 
+import contextlib
 from dataclasses import dataclass
 
 import torch
@@ -53,8 +54,6 @@ class PagedKV4:
             raise ValueError("4-bit pages need at least one head and one row")
         if codes.stride(4) != 1 or scales.stride(5) != 1 or (scales.shape[4] > 1 and scales.stride(4) != 2):
             raise ValueError("the rows of 4-bit pages must be contiguous")
-        if any(st < 0 for st in (*codes.stride(), *scales.stride())):
-            raise ValueError("negative strides")
 
     @classmethod
     def allocate(cls, num_blocks: int, block_size: int, num_heads: int, head_size: int,
@@ -88,17 +87,27 @@ class PagedKV4:
 
     def _pages(self) -> tuple:
         """The pages as the C ABI takes them: pointers and byte strides (block, row, head)."""
-        codes, scales = self.codes, self.scales
-        return (codes[0].data_ptr(), codes[1].data_ptr(), codes.stride(1), codes.stride(3), codes.stride(2),
-                scales[0].data_ptr(), scales[1].data_ptr(), scales.stride(1) * 2, scales.stride(3) * 2,
-                scales.stride(2) * 2)
+        plane, block, head, row, _ = self.codes.stride()
+        s_plane, s_block, s_head, s_row, _, _ = self.scales.stride()
+        codes, scales = self.codes.data_ptr(), self.scales.data_ptr()
+        return (codes, codes + plane, block, row, head, scales, scales + 2 * s_plane, 2 * s_block, 2 * s_row, 2 * s_head)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def on_device(device: torch.device, stream: torch.cuda.Stream | None):
     """Context in which a call allocates and launches: ``stream``, or the device's current stream."""
-    if stream is not None and stream.device != device:
-        raise ValueError(f"the stream belongs to {stream.device}, the tensors to {device}")
-    return torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(device))
+    if stream is not None:
+        if stream.device != device:
+            raise ValueError(f"the stream belongs to {stream.device}, the tensors to {device}")
+        return torch.cuda.stream(stream)
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def current_handle() -> int:
+    """The current device's current stream, without building a Stream object (2 us of a decode call)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _index(name: str, index: torch.Tensor, count: int, device: torch.device, low: int | None, high: int) -> torch.Tensor:
@@ -112,7 +121,9 @@ def _index(name: str, index: torch.Tensor, count: int, device: torch.device, low
             raise IndexError(f"{name} out of range: [{int(index.min())}, {int(index.max())}] for {high}")
     elif index.device.type != "cpu" and index.device != device:
         raise ValueError(f"{name} must live on the host or on {device}")
-    return index.to(device=device, dtype=torch.long).contiguous()
+    if index.dtype != torch.long or index.device != device:
+        index = index.to(device=device, dtype=torch.long)
+    return index.contiguous()
 
 
 def _rows(name: str, tensor: torch.Tensor, like: torch.Tensor) -> None:
@@ -167,7 +178,7 @@ def _append(entry: str, rotary_emb, positions, key, value, query, slot_mapping, 
                      0 if query is None else query.shape[1], heads, head_size, _native.dtype_code(key.dtype),
                      0 if where is None else where.data_ptr(), 0 if table is None else table.data_ptr(), table_code,
                      max_position, rotary_dim, neox, *pages, num_blocks, block_size, slots.data_ptr(),
-                     _native.stream_handle())
+                     current_handle())
         return turned
 
 
@@ -286,5 +297,5 @@ def gather_paged_kv4(
         _native.call("cb_gather_paged_kv4", codes_k, codes_v, block_stride, slot_stride, head_stride, *scales,
                      cache.num_blocks, cache.block_size, cache.num_heads, cache.head_size, slots.data_ptr(), tokens,
                      result.data_ptr(), result.stride(0) * size, result.stride(1) * size, result.stride(2) * size, code,
-                     _native.stream_handle())
+                     current_handle())
         return result

@@ -18,10 +18,8 @@
 // with a NaN or an infinity gets a NaN step, so it reads as NaN.  Two codes to
 // a byte, the lower dimension in the low nibble.
 //
-// What bounds them: HBM at long prompts, the launch at decode sizes.  One
-// thread holds one 16-byte piece of an output row (8 values of a 4-bit row) and
-// reads the partner piece through L1; threads of a block run over one token's
-// pieces first, so rows are read and written whole.
+// What bounds them: HBM at long prompts, the launch at decode sizes.  Threads of
+// a block run over one token's pieces first, so rows are read and written whole.
 #include <algorithm>
 #include <type_traits>
 
@@ -90,6 +88,21 @@ __device__ __forceinline__ void load_n(const T* p, float (&x)[N]) {
     for (int j = 0; j < N; ++j) x[j] = Elem<T>::to_f(p[j]);
   }
 }
+
+// N elements as they lie, in whole 16-byte vectors: loads that are issued before anything
+// that depends on them, in half the registers of fp32.
+template <typename T, int N>
+struct Piece {
+  static constexpr int kVecs = N * static_cast<int>(sizeof(T)) / 16;
+  uint4 v[kVecs];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) v[i] = ld_stream(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ float operator[](int j) const {
+    return Elem<T>::to_f(reinterpret_cast<const T*>(v)[j]);
+  }
+};
 
 template <typename T, int N, bool WIDE>
 __device__ __forceinline__ void store_n(T* p, const float (&y)[N]) {
@@ -167,116 +180,326 @@ __device__ __forceinline__ void rotated(const T* row, int d0, const TAB* table, 
   }
 }
 
-// 8 values of a 4-bit row: the eight lanes of a group agree on its lowest value and step.
-// Every lane of the warp calls this.
-__device__ __forceinline__ uint32_t encode8(const float (&y)[8], __half2& pair) {
-  float low = INFINITY, high = -INFINITY;
-  bool bad = false;
-  float x[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    bad |= (__float_as_uint(y[j]) & 0x7f800000u) == 0x7f800000u;
-    x[j] = fminf(fmaxf(y[j], -kHalfMax), kHalfMax);
-    low = fminf(low, x[j]);
-    high = fmaxf(high, x[j]);
+// Where a thread works: a token, and one piece of HPT heads of K (plane 0), V (1) or Q (2).
+struct Place {
+  bool real;
+  int64_t token;
+  int plane, head, piece;
+};
+template <int HPT, typename P>
+__device__ __forceinline__ Place place(const P& c, int kv_heads, int q_heads, int pieces) {
+  Place w;
+  const int tok = threadIdx.x / c.units_block;
+  const int unit = blockIdx.y * c.units_block + (threadIdx.x - tok * c.units_block);
+  w.token = static_cast<int64_t>(blockIdx.x) * c.tokens_block + tok;
+  w.real = tok < c.tokens_block && unit < c.units && w.token < c.tokens;
+  const int bundles = unit / pieces;  // of HPT heads
+  const int kv_bundles = (kv_heads + HPT - 1) / HPT;
+  w.piece = unit - bundles * pieces;
+  w.plane = bundles < kv_bundles ? 0 : (bundles < 2 * kv_bundles ? 1 : 2);
+  w.head = (bundles - w.plane * kv_bundles) * HPT;
+  return w;
+}
+
+// What a thread does with its token: where its rows go, and whether they go anywhere.
+struct Target {
+  bool turned;  // the position lies inside the table (or nothing is rotated)
+  bool stored;  // K or V with a slot of the cache
+  int64_t position, block, row;
+};
+__device__ __forceinline__ Target target(const Params& c, const Place& w) {
+  Target g{};
+  if (!w.real) return g;
+  const int64_t slot = w.plane < 2 ? __ldg(c.slots + w.token) : -1;
+  g.turned = true;
+  if (c.rotary_dim > 0) {  // V goes with its K: a bad position leaves the whole slot as it was
+    g.position = __ldg(c.positions + w.token);
+    g.turned = g.position >= 0 && g.position < c.max_position;
   }
+  g.stored = slot >= 0 && slot < c.num_slots && g.turned;
+  if (g.stored) split_slot(slot, c.block_size, g.block, g.row);
+  return g;
+}
+
+// 16-byte pieces of 16/32-bit rows.  A thread takes two of them -- for neox the two
+// partners of a rotation, so that each is read once and one piece of the table serves
+// both -- in HPT heads, whose loads are in flight together and share the table's values.
+// HPT 4 at long prompts, 1 where there are too few tokens to fill the GPU (rule and
+// figures at pick_heads).
+template <typename T, typename TAB, int HPT>
+__global__ void __launch_bounds__(kThreads) append_kernel(const Params c) {
+  constexpr int N = 16 / static_cast<int>(sizeof(T));
+  const Place w = place<HPT>(c, c.kv_heads, c.q_heads, c.head_size / (2 * N));
+  if (!w.real) return;
+  const bool is_q = w.plane == 2;
+  const char* src = is_q ? c.query + w.token * c.query_ts
+                         : (w.plane == 0 ? c.key + w.token * c.key_ts : c.value + w.token * c.value_ts);
+  const int64_t src_hs = is_q ? c.query_hs : (w.plane == 0 ? c.key_hs : c.value_hs);
+  const int heads = is_q ? c.q_heads : c.kv_heads;
+  // the two pieces: partners below rotary_dim (neox), neighbours elsewhere
+  const int half = c.rotary_dim >> 1;
+  const bool partners = w.plane != 1 && c.neox && w.piece * N < half;
+  const int d0 = partners ? w.piece * N
+                          : (w.plane != 1 && c.neox ? c.rotary_dim + 2 * (w.piece * N - half) : 2 * w.piece * N);
+  const int d1 = partners ? d0 + half : d0 + N;
+  // padding rows are read too: the loads wait for no slot or position
+  Piece<T, N> a[HPT], b[HPT];
 #pragma unroll
-  for (int o = 4; o >= 1; o >>= 1) {
-    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+  for (int i = 0; i < HPT; ++i)
+    if (w.head + i < heads) {
+      const T* row = reinterpret_cast<const T*>(src + (w.head + i) * src_hs);
+      a[i].load(row + d0);
+      b[i].load(row + d1);
+    }
+  const Target g = target(c, w);
+  if (!is_q && !g.stored) return;
+  float cos[N], sin[N];
+  const bool turn = w.plane != 1 && d0 < c.rotary_dim && g.turned;
+  if (turn) {
+    const TAB* table = static_cast<const TAB*>(c.table) + g.position * c.rotary_dim + (partners ? d0 : d0 / 2);
+    load_n<TAB, N, true>(table, cos);
+    load_n<TAB, N, true>(table + half, sin);
   }
-  const uint32_t votes = __ballot_sync(0xffffffffu, bad);
-  const __half step_h = __float2half_rn(__fmul_rn(__fsub_rn(high, low), 1.0f / 15.0f));
-  const __half low_h = __float2half_rn(low);
-  const float step = __half2float(step_h);
+  char* dst = is_q ? c.query_out + w.token * c.qo_ts
+                   : (w.plane == 0 ? c.k_cache : c.v_cache) + g.block * c.block_stride + g.row * c.slot_stride;
+  const int64_t dst_hs = is_q ? c.qo_hs : c.head_stride;
+#pragma unroll
+  for (int i = 0; i < HPT; ++i)
+    if (w.head + i < heads) {
+      float x[N], y[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) x[j] = g.turned ? a[i][j] : 0.0f, y[j] = g.turned ? b[i][j] : 0.0f;
+      if (turn && partners) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const float p = x[j], q = y[j];
+          x[j] = turn_first(p, q, cos[j], sin[j]);
+          y[j] = turn_second(p, q, cos[j], sin[j]);
+        }
+      } else if (turn) {  // GPT-J: N pairs over the two pieces (rotary_dim is a multiple of both)
+#pragma unroll
+        for (int j = 0; j < N / 2; ++j) {
+          float p = x[2 * j], q = x[2 * j + 1];
+          x[2 * j] = turn_first(p, q, cos[j], sin[j]);
+          x[2 * j + 1] = turn_second(p, q, cos[j], sin[j]);
+          p = y[2 * j], q = y[2 * j + 1];
+          y[2 * j] = turn_first(p, q, cos[N / 2 + j], sin[N / 2 + j]);
+          y[2 * j + 1] = turn_second(p, q, cos[N / 2 + j], sin[N / 2 + j]);
+        }
+      }
+      T* row = reinterpret_cast<T*>(dst + (w.head + i) * dst_hs);
+      store_n<T, N, true>(row + d0, x);
+      store_n<T, N, true>(row + d1, y);
+    }
+}
+
+// Rows that cannot go in aligned 16-byte pieces: a value per thread.
+template <typename T, typename TAB>
+__global__ void __launch_bounds__(kThreads) append_narrow_kernel(const Params c) {
+  const Place w = place<1>(c, c.kv_heads, c.q_heads, c.head_size);
+  if (!w.real) return;
+  const Target g = target(c, w);
+  if (w.plane < 2 && !g.stored) return;
+  const TAB* table = static_cast<const TAB*>(c.table) + g.position * c.rotary_dim;
+  float y[1];
+  T* out;
+  if (w.plane == 2) {
+    out = reinterpret_cast<T*>(c.query_out + w.token * c.qo_ts + w.head * c.qo_hs);
+    if (g.turned)
+      rotated<T, TAB, 1, false>(reinterpret_cast<const T*>(c.query + w.token * c.query_ts + w.head * c.query_hs), w.piece,
+                                table, c.rotary_dim, c.neox != 0, y);
+    else
+      y[0] = 0.0f;
+  } else {
+    out = reinterpret_cast<T*>((w.plane == 0 ? c.k_cache : c.v_cache) + g.block * c.block_stride + g.row * c.slot_stride +
+                               w.head * c.head_stride);
+    if (w.plane == 0)
+      rotated<T, TAB, 1, false>(reinterpret_cast<const T*>(c.key + w.token * c.key_ts + w.head * c.key_hs), w.piece, table,
+                                c.rotary_dim, c.neox != 0, y);
+    else
+      y[0] = Elem<T>::to_f(reinterpret_cast<const T*>(c.value + w.token * c.value_ts + w.head * c.value_hs)[w.piece]);
+  }
+  out[w.piece] = Elem<T>::from_f(y[0]);
+}
+
+// The (step, lowest) pair of a group from its extremes; `bad`: it holds a NaN or an infinity.
+__device__ __forceinline__ __half2 step_of(float low, float high, bool bad) {
+  low = fminf(fmaxf(low, -kHalfMax), kHalfMax);
+  high = fminf(fmaxf(high, -kHalfMax), kHalfMax);
+  const __half step = __float2half_rn(__fmul_rn(__fsub_rn(high, low), 1.0f / 15.0f));
+  return __halves2half2(bad ? __ushort_as_half(0x7e00) : step, __float2half_rn(low));
+}
+// Codes of 8 values, the first in the lowest nibble.
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], __half2 pair) {
+  const float step = __low2float(pair), base = __high2float(pair);
   const float inverse = step > 0.0f ? __frcp_rn(step) : 0.0f;
-  const float base = __half2float(low_h);
   uint32_t codes = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float c = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(x[j], base), inverse)), 0.0f), 15.0f);
-    codes |= static_cast<uint32_t>(c) << (4 * j);
+    const float v = fminf(fmaxf(__fmul_rn(__fsub_rn(x[j], base), inverse), 0.0f), 15.0f);
+    // v + 1.5 * 2^23 has the nearest whole number (ties to even) in its low bits
+    codes |= (__float_as_uint(__fadd_rn(v, 12582912.0f)) & 15u) << (4 * j);
   }
-  const bool group_bad = (votes >> (threadIdx.x & 24u)) & 0xffu;
-  pair = __halves2half2(group_bad ? __ushort_as_half(0x7e00) : step_h, low_h);
   return codes;
 }
 
-// One piece (N values) of one row of K, V or Q per thread.
-template <typename T, typename TAB, int N, bool WIDE, bool FOUR>
-__global__ void __launch_bounds__(kThreads) append_kernel(const Params c) {
-  const int tok = threadIdx.x / c.units_block;
-  const int unit = blockIdx.y * c.units_block + (threadIdx.x - tok * c.units_block);
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * c.tokens_block + tok;
-  const bool real = tok < c.tokens_block && unit < c.units && t < c.tokens;
-  const int pieces = c.head_size / N;
-  const int kv_units = c.kv_heads * pieces;
-  // plane 0: K, 1: V, 2: Q
-  const int plane = unit < kv_units ? 0 : (unit < 2 * kv_units ? 1 : 2);
-  const int in_plane = unit - plane * kv_units;
-  const int head = in_plane / pieces;
-  const int d0 = (in_plane - head * pieces) * N;
-
-  int64_t slot = -1;
-  bool turned = true;  // the position lies inside the table
-  const TAB* table = nullptr;
-  if (real) {
-    if (plane < 2) slot = c.slots[t];
-    if (plane != 1 && c.rotary_dim > 0) {
-      const int64_t pos = c.positions[t];
-      turned = pos >= 0 && pos < c.max_position;
-      table = static_cast<const TAB*>(c.table) + pos * c.rotary_dim;
+// A piece of 8 values rotated in registers: `other` holds a neox rotation's partners.
+__device__ __forceinline__ void turn_piece(float (&x)[8], const float (&other)[8], int d, int rotary, bool neox,
+                                           const float (&cos)[8], const float (&sin)[8]) {
+  if (d >= rotary) return;
+  if (neox) {
+    const bool first = d < (rotary >> 1);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      x[j] = first ? turn_first(x[j], other[j], cos[j], sin[j]) : turn_second(other[j], x[j], cos[j], sin[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float p = x[2 * j], q = x[2 * j + 1];
+      x[2 * j] = turn_first(p, q, cos[j], sin[j]);
+      x[2 * j + 1] = turn_second(p, q, cos[j], sin[j]);
     }
   }
-  // V goes with its K: a position outside the table leaves the whole slot as it was
-  if (real && plane == 1 && c.rotary_dim > 0) {
-    const int64_t pos = c.positions[t];
-    turned = pos >= 0 && pos < c.max_position;
+}
+
+// 4-bit rows.  A lane takes the 8-value pieces at 8 p and D / 2 + 8 p of HPT heads of K or V
+// (and of the queries, which stay of their type): the two partners of a neox rotation over
+// the whole head, so nothing is read twice, and for D 128 one piece of each group of 64.  The
+// eight lanes of a D 128 row reduce both groups side by side, the four of a D 64 row their one.
+// EXTRA: neox over a part of the head, whose partners are read beside (they come from L1).
+// !WIDE: rows that are not aligned, or a rotary_dim that cuts a piece, value by value.
+template <typename T, typename TAB, int D, bool WIDE, bool EXTRA, int HPT>
+__global__ void __launch_bounds__(kThreads) append4_kernel(const Params c) {
+  const Place w = place<HPT>(c, c.kv_heads, c.q_heads, D / 16);
+  const bool is_q = w.plane == 2, neox = c.neox != 0;
+  const char* src = is_q ? c.query + w.token * c.query_ts
+                         : (w.plane == 0 ? c.key + w.token * c.key_ts : c.value + w.token * c.value_ts);
+  const int64_t src_hs = is_q ? c.query_hs : (w.plane == 0 ? c.key_hs : c.value_hs);
+  const int heads = w.real ? (is_q ? c.q_heads : c.kv_heads) : 0;
+  const int half = c.rotary_dim >> 1;
+  const int at[2] = {8 * w.piece, D / 2 + 8 * w.piece};
+  int with[2];  // partners of the two pieces
+#pragma unroll
+  for (int s = 0; s < 2; ++s) with[s] = at[s] >= c.rotary_dim ? at[s] : (at[s] < half ? at[s] + half : at[s] - half);
+  // padding rows are read too: the loads wait for no slot or position
+  Piece<T, 8> own[HPT][2], beside[EXTRA ? HPT : 1][2];
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int i = 0; i < HPT; ++i)
+      if (w.head + i < heads) {
+        const T* row = reinterpret_cast<const T*>(src + (w.head + i) * src_hs);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          own[i][s].load(row + at[s]);
+          if constexpr (EXTRA) beside[i][s].load(row + with[s]);
+        }
+      }
   }
-  const bool stored = real && plane < 2 && slot >= 0 && slot < c.num_slots && turned;
-  float y[N];
-  if (real && plane == 2) {
-    T* out = reinterpret_cast<T*>(c.query_out + t * c.qo_ts + head * c.qo_hs) + d0;
-    if (turned) {
-      rotated<T, TAB, N, WIDE>(reinterpret_cast<const T*>(c.query + t * c.query_ts + head * c.query_hs), d0, table,
-                               c.rotary_dim, c.neox != 0, y);
+  const Target g = target(c, w);
+  const bool turn = w.plane != 1 && c.rotary_dim > 0 && g.turned;
+  const TAB* table = static_cast<const TAB*>(c.table) + g.position * c.rotary_dim;
+  float cos[2][8], sin[2][8];
+  if constexpr (WIDE) {
+    if (turn) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (neox) {
+          const int i = at[s] < half ? at[s] : with[s];
+          if (at[s] < c.rotary_dim) {
+            load_n<TAB, 8, true>(table + i, cos[s]);
+            load_n<TAB, 8, true>(table + half + i, sin[s]);
+          }
+        } else if (at[s] < c.rotary_dim) {
+          float few[4];
+          load_n<TAB, 4, true>(table + at[s] / 2, few);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) cos[s][j] = few[j];
+          load_n<TAB, 4, true>(table + half + at[s] / 2, few);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sin[s][j] = few[j];
+        }
+      }
+    }
+  }
+  const int64_t row_at = g.block * c.block_stride + g.row * c.slot_stride;
+  const int64_t scale_at = g.block * c.scale_block_stride + g.row * c.scale_slot_stride;
+#pragma unroll
+  for (int i = 0; i < HPT; ++i) {
+    const bool here = w.head + i < heads && (is_q || g.stored);
+    float x[2][8];
+    if (here && g.turned) {
+      if constexpr (WIDE) {
+        float other[2][8];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            x[s][j] = own[i][s][j];
+            other[s][j] = EXTRA ? beside[EXTRA ? i : 0][s][j] : own[i][1 - s][j];
+          }
+        if (turn) {
+#pragma unroll
+          for (int s = 0; s < 2; ++s) turn_piece(x[s], other[s], at[s], c.rotary_dim, neox, cos[s], sin[s]);
+        }
+      } else {
+        const T* row = reinterpret_cast<const T*>(src + (w.head + i) * src_hs);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) rotated<T, TAB, 8, false>(row, at[s], table, turn ? c.rotary_dim : 0, neox, x[s]);
+      }
     } else {
 #pragma unroll
-      for (int j = 0; j < N; ++j) y[j] = 0.0f;
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[s][j] = 0.0f;
     }
-    store_n<T, N, WIDE>(out, y);
-  } else if (stored) {
-    if (plane == 0)
-      rotated<T, TAB, N, WIDE>(reinterpret_cast<const T*>(c.key + t * c.key_ts + head * c.key_hs), d0, table,
-                               c.rotary_dim, c.neox != 0, y);
-    else
-      load_n<T, N, WIDE>(reinterpret_cast<const T*>(c.value + t * c.value_ts + head * c.value_hs) + d0, y);
-  } else {
+    if (here && is_q) {
+      T* out = reinterpret_cast<T*>(c.query_out + w.token * c.qo_ts + (w.head + i) * c.qo_hs);
 #pragma unroll
-    for (int j = 0; j < N; ++j) y[j] = 0.0f;
-  }
-  if constexpr (!FOUR) {
-    if (!stored) return;
-    int64_t block, row;
-    split_slot(slot, c.block_size, block, row);
-    char* dst = (plane == 0 ? c.k_cache : c.v_cache) + block * c.block_stride + row * c.slot_stride + head * c.head_stride;
-    store_n<T, N, WIDE>(reinterpret_cast<T*>(dst) + d0, y);
-  } else {
-    static_assert(N == 8, "eight lanes to a group of 64");
-    // the row as the element type holds it: the 4-bit pages hold what 16-bit pages would
+      for (int s = 0; s < 2; ++s) store_n<T, 8, WIDE>(out + at[s], x[s]);
+    }
+    float low[2], high[2], odd[2];
 #pragma unroll
-    for (int j = 0; j < N; ++j) y[j] = rnd<T>(y[j]);
-    __half2 pair;
-    const uint32_t codes = encode8(y, pair);
-    if (!stored) return;
-    int64_t block, row;
-    split_slot(slot, c.block_size, block, row);
-    char* dst = (plane == 0 ? c.k_cache : c.v_cache) + block * c.block_stride + row * c.slot_stride + head * c.head_stride;
-    *reinterpret_cast<uint32_t*>(dst + d0 / 2) = codes;
-    if ((d0 & (kGroup - 1)) == 0) {
-      char* sc = (plane == 0 ? c.k_scales : c.v_scales) + block * c.scale_block_stride + row * c.scale_slot_stride +
-                 head * c.scale_head_stride;
-      *(reinterpret_cast<__half2*>(sc) + d0 / kGroup) = pair;
+    for (int s = 0; s < 2; ++s) {
+      low[s] = INFINITY, high[s] = -INFINITY, odd[s] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        // the row as the element type holds it: 4-bit pages hold what 16-bit pages would
+        x[s][j] = rnd<T>(x[s][j]);
+        low[s] = fminf(low[s], x[s][j]);
+        high[s] = fmaxf(high[s], x[s][j]);
+        odd[s] = fmaf(x[s][j], 0.0f, odd[s]);  // NaN once a value is NaN or infinite
+      }
+    }
+    if constexpr (D == 64) {
+      low[0] = fminf(low[0], low[1]), high[0] = fmaxf(high[0], high[1]), odd[0] += odd[1];
+    }
+    // every lane of the warp is here: the lanes of a row reduce with their neighbours
+    constexpr int kGroups = D / kGroup;
+    __half2 pair[2];
+#pragma unroll
+    for (int s = 0; s < kGroups; ++s) {
+#pragma unroll
+      for (int o = D / 32; o >= 1; o >>= 1) {
+        low[s] = fminf(low[s], __shfl_xor_sync(0xffffffffu, low[s], o));
+        high[s] = fmaxf(high[s], __shfl_xor_sync(0xffffffffu, high[s], o));
+      }
+      const uint32_t votes = __ballot_sync(0xffffffffu, odd[s] != 0.0f);  // unequal also when NaN
+      constexpr uint32_t kLanes = D / 16;
+      pair[s] = step_of(low[s], high[s], (votes >> (threadIdx.x & (32u - kLanes))) & ((1u << kLanes) - 1u));
+    }
+    if constexpr (D == 64) pair[1] = pair[0];
+    if (!here || is_q) continue;
+    char* dst = (w.plane == 0 ? c.k_cache : c.v_cache) + row_at + (w.head + i) * c.head_stride;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) *reinterpret_cast<uint32_t*>(dst + at[s] / 2) = codes_of(x[s], pair[s]);
+    if (w.piece == 0) {
+      char* sc = (w.plane == 0 ? c.k_scales : c.v_scales) + scale_at + (w.head + i) * c.scale_head_stride;
+      if constexpr (D == 64) {
+        *reinterpret_cast<__half2*>(sc) = pair[0];
+      } else {
+        *reinterpret_cast<uint2*>(sc) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&pair[0]), *reinterpret_cast<const uint32_t*>(&pair[1]));
+      }
     }
   }
 }
@@ -297,36 +520,44 @@ struct GatherParams {
   int units, units_block, tokens_block;
 };
 
-// 8 values of one row of K or V per thread; a slot outside the cache reads as zeros.
-template <typename T, bool WIDE>
+// 16 values of HPT heads of K or V per thread; a slot outside the cache reads as zeros.
+template <typename T, bool WIDE, int HPT>
 __global__ void __launch_bounds__(kThreads) gather4_kernel(const GatherParams c) {
-  const int tok = threadIdx.x / c.units_block;
-  const int unit = blockIdx.y * c.units_block + (threadIdx.x - tok * c.units_block);
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * c.tokens_block + tok;
-  if (tok >= c.tokens_block || unit >= c.units || t >= c.tokens) return;
-  const int pieces = c.head_size / 8;
-  const int row_piece = unit / pieces;
-  const int d0 = (unit - row_piece * pieces) * 8;
-  const int plane = row_piece >= c.heads;
-  const int head = row_piece - plane * c.heads;
-  const int64_t slot = c.slots[t];
-  float y[8];
+  const Place w = place<HPT>(c, c.heads, 0, c.head_size / 16);
+  if (!w.real) return;
+  const int64_t slot = __ldg(c.slots + w.token);
+  const int d0 = w.piece * 16;
+  uint2 codes[HPT];
+  float2 pair[HPT];
+#pragma unroll
+  for (int i = 0; i < HPT; ++i) codes[i] = make_uint2(0, 0), pair[i] = make_float2(0.0f, 0.0f);
   if (slot >= 0 && slot < c.num_slots) {
     int64_t block, row;
     split_slot(slot, c.block_size, block, row);
-    const char* src = (plane ? c.v_codes : c.k_codes) + block * c.block_stride + row * c.slot_stride + head * c.head_stride;
-    const char* sc = (plane ? c.v_scales : c.k_scales) + block * c.scale_block_stride + row * c.scale_slot_stride +
-                     head * c.scale_head_stride;
-    const uint32_t codes = __ldg(reinterpret_cast<const uint32_t*>(src + d0 / 2));
-    const float2 pair = __half22float2(__ldg(reinterpret_cast<const __half2*>(sc) + d0 / kGroup));
+    const char* src = (w.plane ? c.v_codes : c.k_codes) + block * c.block_stride + row * c.slot_stride + d0 / 2;
+    const char* sc = (w.plane ? c.v_scales : c.k_scales) + block * c.scale_block_stride + row * c.scale_slot_stride +
+                     d0 / kGroup * static_cast<int>(sizeof(__half2));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = fmaf(static_cast<float>((codes >> (4 * j)) & 15u), pair.x, pair.y);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = 0.0f;
+    for (int i = 0; i < HPT; ++i)
+      if (w.head + i < c.heads) {
+        codes[i] = __ldg(reinterpret_cast<const uint2*>(src + (w.head + i) * c.head_stride));
+        pair[i] = __half22float2(__ldg(reinterpret_cast<const __half2*>(sc + (w.head + i) * c.scale_head_stride)));
+      }
   }
-  store_n<T, 8, WIDE>(
-      reinterpret_cast<T*>(c.out + plane * c.out_plane_stride + t * c.out_token_stride + head * c.out_head_stride) + d0, y);
+  T* out = reinterpret_cast<T*>(c.out + w.plane * c.out_plane_stride + w.token * c.out_token_stride) + d0;
+#pragma unroll
+  for (int i = 0; i < HPT; ++i)
+    if (w.head + i < c.heads) {
+      T* row = reinterpret_cast<T*>(reinterpret_cast<char*>(out) + (w.head + i) * c.out_head_stride);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const uint32_t word = s ? codes[i].y : codes[i].x;
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = fmaf(static_cast<float>((word >> (4 * j)) & 15u), pair[i].x, pair[i].y);
+        store_n<T, 8, WIDE>(row + 8 * s, y);
+      }
+    }
 }
 
 // Threads of a block: the units of one token, or of several tokens side by side.
@@ -339,18 +570,55 @@ dim3 lay_out(P& c, int64_t units, int64_t tokens) {
               static_cast<unsigned>((units + c.units_block - 1) / c.units_block));
 }
 
+// Units of a token: pieces of bundles of `hpt` heads.
+inline int64_t units_of(int64_t kv_heads, int64_t q_heads, int64_t pieces, int64_t hpt) {
+  return (2 * ((kv_heads + hpt - 1) / hpt) + (q_heads + hpt - 1) / hpt) * pieces;
+}
+
+// Whether a thread takes four heads: once one head per thread would fill the GPU's resident
+// threads anyway.
+inline bool four_heads(int64_t units, int64_t tokens) { return units * tokens >= int64_t(kSmCount) * 2048; }
+
+int check_units(int64_t units) {
+  CB_REQUIRE(units < (int64_t(1) << 23), "row too wide (%lld pieces)", (long long)units);
+  return CB_OK;
+}
+
+template <typename T, typename TAB, int D>
+void launch4(const Params& c, dim3 grid, bool wide, bool four, cudaStream_t s) {
+  const bool extra = c.neox && c.rotary_dim > 0 && c.rotary_dim < D;
+  if (!wide)
+    append4_kernel<T, TAB, D, false, false, 1><<<grid, kThreads, 0, s>>>(c);
+  else if (extra)
+    four ? append4_kernel<T, TAB, D, true, true, 4><<<grid, kThreads, 0, s>>>(c)
+         : append4_kernel<T, TAB, D, true, true, 1><<<grid, kThreads, 0, s>>>(c);
+  else
+    four ? append4_kernel<T, TAB, D, true, false, 4><<<grid, kThreads, 0, s>>>(c)
+         : append4_kernel<T, TAB, D, true, false, 1><<<grid, kThreads, 0, s>>>(c);
+}
+
 template <bool FOUR, typename T, typename TAB>
 int launch(Params& c, bool wide, cudaStream_t s) {
-  constexpr int kWide = FOUR ? 8 : 16 / static_cast<int>(sizeof(T));
-  constexpr int kNarrow = FOUR ? 8 : 1;
-  const int64_t n = wide ? kWide : kNarrow;
-  const int64_t units = (2 * static_cast<int64_t>(c.kv_heads) + c.q_heads) * (c.head_size / n);
-  CB_REQUIRE(units < (int64_t(1) << 23), "row too wide (%lld pieces)", (long long)units);
-  const dim3 grid = lay_out(c, units, c.tokens);
-  if (wide)
-    append_kernel<T, TAB, kWide, true, FOUR><<<grid, kThreads, 0, s>>>(c);
-  else
-    append_kernel<T, TAB, kNarrow, false, FOUR><<<grid, kThreads, 0, s>>>(c);
+  constexpr int kPiece = FOUR ? 16 : 32 / static_cast<int>(sizeof(T));
+  const int64_t pieces = FOUR || wide ? c.head_size / kPiece : c.head_size;
+  const int64_t units = units_of(c.kv_heads, c.q_heads, pieces, 1);
+  const int rc = check_units(units);
+  if (rc != CB_OK) return rc;
+  const bool four = wide && four_heads(units, c.tokens);
+  const dim3 grid = lay_out(c, four ? units_of(c.kv_heads, c.q_heads, pieces, 4) : units, c.tokens);
+  if constexpr (FOUR) {
+    if (c.head_size == 64)
+      launch4<T, TAB, 64>(c, grid, wide, four, s);
+    else
+      launch4<T, TAB, 128>(c, grid, wide, four, s);
+  } else {
+    if (!wide)
+      append_narrow_kernel<T, TAB><<<grid, kThreads, 0, s>>>(c);
+    else if (four)
+      append_kernel<T, TAB, 4><<<grid, kThreads, 0, s>>>(c);
+    else
+      append_kernel<T, TAB, 1><<<grid, kThreads, 0, s>>>(c);
+  }
   return launch_status(FOUR ? "cb_append_paged_kv4" : "cb_append_paged_kv");
 }
 
@@ -365,6 +633,19 @@ int dispatch(Params& c, int dtype, int table_dtype, bool wide, cudaStream_t s) {
     default:
       return launch<FOUR, float, float>(c, wide, s);
   }
+}
+
+template <typename T>
+void launch_gather4(GatherParams& c, bool wide, cudaStream_t s) {
+  const int64_t pieces = c.head_size / 16, units = units_of(c.heads, 0, pieces, 1);
+  const bool four = wide && four_heads(units, c.tokens);
+  const dim3 grid = lay_out(c, four ? units_of(c.heads, 0, pieces, 4) : units, c.tokens);
+  if (!wide)
+    gather4_kernel<T, false, 1><<<grid, kThreads, 0, s>>>(c);
+  else if (four)
+    gather4_kernel<T, true, 4><<<grid, kThreads, 0, s>>>(c);
+  else
+    gather4_kernel<T, true, 1><<<grid, kThreads, 0, s>>>(c);
 }
 
 // What both appends check of their rows and of the rotation.
@@ -394,15 +675,14 @@ int check_rows(const Params& c, int dtype, int table_dtype, int64_t num_blocks) 
   return CB_OK;
 }
 
-// Whether pieces of `n` values can be read whole: aligned rows, and no piece across
-// rotary_dim or (neox) its half.  Rows that cannot go value by value; measured for one
-// 8,192-token prompt of 8 KV heads beside the wide form: see below the launch.
-bool wide_rows(const Params& c, int n, uint64_t more) {
+// Whether rows go in whole aligned pieces: `n` values a piece, `row` values a multiple of
+// which a head holds, and no piece across rotary_dim or (neox) its half.
+bool wide_rows(const Params& c, int n, int row, uint64_t more) {
   const uint64_t acc = more | reinterpret_cast<uint64_t>(c.key) | reinterpret_cast<uint64_t>(c.value) |
                        reinterpret_cast<uint64_t>(c.query) | reinterpret_cast<uint64_t>(c.query_out) | (uint64_t)c.key_ts |
                        (uint64_t)c.key_hs | (uint64_t)c.value_ts | (uint64_t)c.value_hs | (uint64_t)c.query_ts |
                        (uint64_t)c.query_hs | (uint64_t)c.qo_ts | (uint64_t)c.qo_hs | reinterpret_cast<uint64_t>(c.table);
-  if ((acc & 15u) != 0 || c.head_size % n != 0) return false;
+  if ((acc & 15u) != 0 || c.head_size % row != 0) return false;
   return c.neox ? c.rotary_dim % (2 * n) == 0 : c.rotary_dim % n == 0 && (c.rotary_dim / 2) % n == 0;
 }
 
@@ -457,7 +737,8 @@ extern "C" int cb_append_paged_kv(const void* key, int64_t key_token_stride, int
   const uint64_t pages = reinterpret_cast<uint64_t>(k_cache) | reinterpret_cast<uint64_t>(v_cache) | (uint64_t)block_stride |
                          (uint64_t)slot_stride | (uint64_t)head_stride;
   CB_REQUIRE((pages & (uint64_t)(dtype_bytes(dtype) - 1)) == 0, "pages must be aligned to their element size");
-  const bool wide = append::wide_rows(c, 16 / dtype_bytes(dtype), pages);
+  const int piece = 16 / dtype_bytes(dtype);
+  const bool wide = append::wide_rows(c, piece, 2 * piece, pages);
   return append::dispatch<false>(c, dtype, cos_sin_dtype, wide, reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -495,7 +776,7 @@ extern "C" int cb_append_paged_kv4(const void* key, int64_t key_token_stride, in
   rc = append::check_pages4(block_stride, slot_stride, head_stride, scale_block_stride, scale_slot_stride,
                             scale_head_stride, k_codes, v_codes, k_scales, v_scales, head_size);
   if (rc != CB_OK) return rc;
-  return append::dispatch<true>(c, dtype, cos_sin_dtype, append::wide_rows(c, 8, 0), reinterpret_cast<cudaStream_t>(stream));
+  return append::dispatch<true>(c, dtype, cos_sin_dtype, append::wide_rows(c, 8, 16, 0), reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" int cb_gather_paged_kv4(const void* k_codes, const void* v_codes, int64_t block_stride, int64_t slot_stride,
@@ -528,22 +809,15 @@ extern "C" int cb_gather_paged_kv4(const void* k_codes, const void* v_codes, int
   c.heads = static_cast<int>(num_heads), c.head_size = static_cast<int>(head_size);
   c.slots = slots, c.tokens = num_tokens, c.out = static_cast<char*>(out);
   c.out_plane_stride = out_plane_stride, c.out_token_stride = out_token_stride, c.out_head_stride = out_head_stride;
-  const dim3 grid = append::lay_out(c, 2 * num_heads * (head_size / 8), num_tokens);
+  rc = append::check_units(append::units_of(num_heads, 0, head_size / 16, 1));
+  if (rc != CB_OK) return rc;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const bool wide = (acc & 15u) == 0;
-  switch (dtype) {
-    case CB_DTYPE_BF16:
-      wide ? append::gather4_kernel<__nv_bfloat16, true><<<grid, append::kThreads, 0, s>>>(c)
-           : append::gather4_kernel<__nv_bfloat16, false><<<grid, append::kThreads, 0, s>>>(c);
-      break;
-    case CB_DTYPE_FP16:
-      wide ? append::gather4_kernel<__half, true><<<grid, append::kThreads, 0, s>>>(c)
-           : append::gather4_kernel<__half, false><<<grid, append::kThreads, 0, s>>>(c);
-      break;
-    default:
-      wide ? append::gather4_kernel<float, true><<<grid, append::kThreads, 0, s>>>(c)
-           : append::gather4_kernel<float, false><<<grid, append::kThreads, 0, s>>>(c);
-      break;
-  }
+  if (dtype == CB_DTYPE_BF16)
+    append::launch_gather4<__nv_bfloat16>(c, wide, s);
+  else if (dtype == CB_DTYPE_FP16)
+    append::launch_gather4<__half>(c, wide, s);
+  else
+    append::launch_gather4<float>(c, wide, s);
   return launch_status("cb_gather_paged_kv4");
 }
