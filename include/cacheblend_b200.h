@@ -496,6 +496,38 @@ CB_API int cb_gather_paged_kv4(const void* k_codes, const void* v_codes, int64_t
                                void* out, int64_t out_plane_stride, int64_t out_token_stride,
                                int64_t out_head_stride, int dtype, void* stream);
 
+/*
+ * Attention of the newest tokens of each sequence over 4-bit pages, causal:
+ * sequence i owns the query rows query_start[i] .. query_start[i + 1] - 1 (NULL:
+ * row i alone, num_tokens == num_seqs) and the first seq_lens[i] keys that its
+ * row of block_table [num_seqs][table_width] (rows table_stride entries apart)
+ * names, those of the query tokens included: token j of n sees the keys at or
+ * before seq_lens[i] - n + j.  query and out: [num_tokens][num_q_heads]
+ * [head_size] bf16 or fp16 with token and head strides (bytes); query head h
+ * attends KV head h / (num_q_heads / num_kv_heads).  Keys past the table's width
+ * and pages outside the cache are left out; a row that sees no key is zeros;
+ * rows of no sequence are not written; query_start is clamped to the rows there
+ * are.  Logits, softmax and sums in fp32, the weighted steps of the values
+ * rounded to fp16 before the product with their codes.  `workspace`: 16-byte
+ * aligned device memory of cb_paged_attention4_workspace_size bytes, any
+ * contents; calls that share one must not overlap on the GPU.
+ */
+CB_API int cb_paged_attention4_workspace_size(int64_t num_tokens, int64_t num_seqs,
+                                              int64_t num_q_heads, int64_t num_kv_heads,
+                                              int64_t head_size, int64_t* bytes);
+CB_API int cb_paged_attention4(const void* query, int64_t query_token_stride,
+                               int64_t query_head_stride, int64_t num_tokens, int64_t num_q_heads,
+                               int dtype, const int32_t* query_start, const void* k_codes,
+                               const void* v_codes, int64_t block_stride, int64_t slot_stride,
+                               int64_t head_stride, const void* k_scales, const void* v_scales,
+                               int64_t scale_block_stride, int64_t scale_slot_stride,
+                               int64_t scale_head_stride, int64_t num_blocks, int64_t block_size,
+                               int64_t num_kv_heads, int64_t head_size, const int32_t* block_table,
+                               int64_t table_stride, int64_t table_width, const int32_t* seq_lens,
+                               int64_t num_seqs, float scale, void* out, int64_t out_token_stride,
+                               int64_t out_head_stride, void* workspace, int64_t workspace_bytes,
+                               void* stream);
+
 #ifdef __cplusplus
 }
 #endif

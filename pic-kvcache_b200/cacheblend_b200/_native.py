@@ -151,6 +151,13 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_ptr, _ptr, _i64, _i64, _i64, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _ptr,
          _i64, _ptr, _i64, _i64, _i64, _i32, _ptr],
     ),
+    "cb_paged_attention4_workspace_size": (_i32, [_i64, _i64, _i64, _i64, _i64, _ptr]),
+    "cb_paged_attention4": (
+        _i32,
+        [_ptr, _i64, _i64, _i64, _i64, _i32, _ptr, _ptr, _ptr, _i64, _i64, _i64, _ptr, _ptr, _i64,
+         _i64, _i64, _i64, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, ctypes.c_float, _ptr, _i64,
+         _i64, _ptr, _i64, _ptr],
+    ),
 }
 
 _lock = threading.Lock()

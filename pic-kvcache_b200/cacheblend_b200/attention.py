@@ -1,10 +1,10 @@
-"""Blend attention on the tensor cores (cb_blend_attention).
+"""Attention: of a blend request's staging, and of decode steps over 4-bit pages.
 
-The side executor's attention of the computed, possibly pruned, queries over
+Blend attention on the tensor cores (cb_blend_attention): the side executor's attention of the computed, possibly pruned, queries over
 the whole staging context: Qwen3BlendExecutor._attention
 (cacheblend_vllm/ascend.py:798-846).  Queries sit at absolute positions and
 attend every staging row at or before their position; grouped query heads
-share their KV head.
+share their KV head.  ``paged_attention4``: at the end of the file.
 """
 
 from __future__ import annotations
@@ -14,6 +14,7 @@ import ctypes
 import torch
 
 from . import _native
+from .append import PagedKV4, current_handle, on_device
 
 
 # exact_rounding argument -> the C ABI's mode code
@@ -97,3 +98,97 @@ def blend_attention(
         0 if device_error is None else device_error.data_ptr(), _native.stream_handle(stream),
     )
     return out
+
+
+def _int32(name: str, tensor: torch.Tensor, device: torch.device, ndim: int) -> None:
+    if tensor.dtype != torch.int32 or tensor.device != device or tensor.ndim != ndim:
+        raise ValueError(f"{name} must be a {ndim}-dimensional int32 tensor on {device}")
+    if tensor.shape[-1] > 1 and tensor.stride(-1) != 1:
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _attention_out(query: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
+    if out is None:
+        return torch.empty_like(query, memory_format=torch.contiguous_format)
+    if out.shape != query.shape or out.dtype != query.dtype or out.device != query.device:
+        raise ValueError("out must match the query's shape, dtype and device")
+    if out.stride(2) != 1:
+        raise ValueError("out heads must be contiguous")
+    return out
+
+
+def paged_attention4_workspace_bytes(num_tokens: int, num_seqs: int, num_q_heads: int, num_kv_heads: int,
+                                     head_size: int) -> int:
+    size = ctypes.c_int64(0)
+    _native.call("cb_paged_attention4_workspace_size", num_tokens, num_seqs, num_q_heads, num_kv_heads, head_size,
+                 ctypes.addressof(size))
+    return int(size.value)
+
+
+def paged_attention4(
+    query: torch.Tensor,
+    cache: PagedKV4,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    scale: float,
+    query_start: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+    stream: torch.cuda.Stream | None = None,
+) -> torch.Tensor:
+    """Causal attention of each sequence's newest tokens over its 4-bit pages: ``[tokens, q_heads, head]``.
+
+    ``query``: ``[tokens, q_heads, head_size]`` bf16 or fp16; query head h attends KV head
+    ``h // (q_heads // kv_heads)``.  ``block_table``: int32 ``[seqs, pages]``, the pages of each
+    sequence in order; ``seq_lens``: int32 ``[seqs]``, its keys, those of the query tokens
+    included (append them first).  One token per sequence, or ``query_start``: int32
+    ``[seqs + 1]``, where each sequence's rows begin; token j of n sees the keys at or before
+    ``seq_lens - n + j``.
+
+    A row that sees no key (an empty sequence) is zeros; rows behind the last sequence are left
+    as ``out`` held them.  Pages outside the cache and keys past the table's width are left
+    out.  ``workspace``: ``paged_attention4_workspace_bytes`` of uint8, for callers that keep one
+    (two calls that may overlap need two); otherwise allocated per call.
+    """
+    if query.ndim != 3:
+        raise ValueError("query must be [tokens, q_heads, head_size]")
+    if query.dtype not in (torch.bfloat16, torch.float16):
+        raise NotImplementedError(f"queries must be bfloat16 or float16, not {query.dtype}")
+    tokens, heads, head_size = query.shape
+    if head_size != cache.head_size or heads == 0 or heads % cache.num_heads:
+        raise ValueError(f"query {tuple(query.shape)} does not fit {cache.num_heads} KV heads of {cache.head_size}")
+    if query.stride(2) != 1:
+        raise ValueError("query heads must be contiguous")
+    device = query.device
+    if cache.device != device:
+        raise ValueError("query and cache must live on one device")
+    _int32("block_table", block_table, device, 2)
+    _int32("seq_lens", seq_lens, device, 1)
+    seqs = seq_lens.shape[0]
+    if block_table.shape[0] != seqs:
+        raise ValueError("block_table must hold one row per sequence")
+    if query_start is not None:
+        _int32("query_start", query_start, device, 1)
+        if query_start.shape[0] != seqs + 1:
+            raise ValueError("query_start must hold one entry per sequence and one more")
+    elif tokens != seqs:
+        raise ValueError(f"{tokens} query tokens for {seqs} sequences need query_start")
+    _native.require_cuda(query)
+    with on_device(device, stream):
+        result = _attention_out(query, out)
+        if tokens == 0 or seqs == 0:
+            return result
+        need = paged_attention4_workspace_bytes(tokens, seqs, heads, cache.num_heads, head_size)
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        elif workspace.dtype != torch.uint8 or workspace.device != device or not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous uint8 on the query's device")
+        token, row, _ = query.stride()
+        out_token, out_row, _ = result.stride()
+        _native.call(
+            "cb_paged_attention4", query.data_ptr(), 2 * token, 2 * row, tokens, heads,
+            _native.DTYPE_CODES[query.dtype], 0 if query_start is None else query_start.data_ptr(), *cache._pages(),
+            cache.num_blocks, cache.block_size, cache.num_heads, head_size,
+            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), seqs, float(scale),
+            result.data_ptr(), 2 * out_token, 2 * out_row, workspace.data_ptr(), workspace.numel(), current_handle())
+        return result

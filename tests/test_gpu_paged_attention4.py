@@ -1,0 +1,255 @@
+"""cb_paged_attention4 against attention in 64 bits over the values that the pages hold.
+
+Bound, per output with probabilities p_j (exact), values v_j = low_j + step_j c_j and
+u = eps / 2 of the output type:
+
+* a factor p step' is rounded to fp16: 2^-11 relative, so at most 2^-11 sum p step' c
+  (below 2^-14 it is a subnormal: the reference keeps the largest of a call's factors
+  over 2^-5, so such a factor is off by 2^-25 / 2^-5 = 2^-20 of the largest p step',
+  which over n keys is at most n 2^-20 15 max(p step'));
+* exp2, the fp32 sums and the logits: a logit is a sum of 2 x 64 products over fp32 with
+  terms of size A = scale log2e sum |q| |k| (codes and lowest value apart), off by at most
+  2^-24 (128 + 8) A, which changes p by that much relative: 2^-16 A;
+* the result is rounded once: u |out|.
+
+    |got - want| <= u |want| + (2^-11 + 2^-15 A) sum p (step c + |low|) + n 2^-16 max(p step) + tiny
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from cacheblend_b200 import PagedKV4, append_paged_kv4, gather_paged_kv4, paged_attention4
+from cacheblend_b200.attention import paged_attention4_workspace_bytes
+
+pytestmark = pytest.mark.gpu
+
+
+def _pages(device, lens, block, kv_heads, head, seed, step=(0.15, 0.35), low=(-2.7, -1.2), spare=2):
+    """(cache with random pages, block table) for sequences of ``lens`` keys."""
+    gen = torch.Generator().manual_seed(seed)
+    pages = [-(-n // block) for n in lens]
+    blocks = sum(pages) + spare
+    order = torch.randperm(blocks, generator=gen).to(torch.int32)
+    table = torch.full((len(lens), max(max(pages), 1) + 1), -1, dtype=torch.int32)  # unused entries are padding
+    at = 0
+    for i, n in enumerate(pages):
+        table[i, :n] = order[at:at + n]
+        at += n
+    codes = torch.randint(0, 256, (2, blocks, kv_heads, block, head // 2), generator=gen, dtype=torch.uint8)
+    pairs = torch.rand(2, blocks, kv_heads, block, head // 64, 2, generator=gen)
+    pairs[..., 0] = step[0] + pairs[..., 0] * (step[1] - step[0])
+    pairs[..., 1] = low[0] + pairs[..., 1] * (low[1] - low[0])
+    pairs = pairs.half()
+    for i, n in enumerate(lens):  # rows behind a sequence's end: whatever memory held
+        if n % block:
+            pairs[:, table[i, n // block], :, n % block:] = torch.nan
+            codes[:, table[i, n // block], :, n % block:] = 255
+    return PagedKV4(codes.to(device), pairs.to(device)), table.to(device)
+
+
+def _parts(cache, table_row, n, plane):
+    """(step * code, low) in 64 bits, [n, kv_heads, head]."""
+    block = cache.block_size
+    pages = table_row[:-(-n // block)].long()
+    codes = cache.codes[plane][pages]
+    codes = torch.stack((codes & 15, codes >> 4), -1).flatten(-2).double().unflatten(-1, (-1, 64))
+    pair = cache.scales[plane][pages].double()
+    varied, low = codes * pair[..., :1], pair[..., 1:].expand_as(codes)
+    order = lambda x: x.flatten(-2).transpose(1, 2).flatten(0, 1)[:n]  # noqa: E731
+    return order(varied), order(low)
+
+
+def _check(got, query, cache, table, lens, scale, start=None):
+    groups = query.shape[1] // cache.num_heads
+    info = torch.finfo(query.dtype)
+    worst = 0.0
+    for i, n in enumerate(lens):
+        a, b = (start[i], start[i + 1]) if start is not None else (i, i + 1)
+        if n == 0:
+            assert int((got[a:b] != 0).sum()) == 0
+            continue
+        kv, kl = _parts(cache, table[i], n, 0)
+        vv, vl = _parts(cache, table[i], n, 1)
+        for j in range(a, b):
+            seen = n - (b - a) + (j - a) + 1
+            if seen <= 0:
+                assert int((got[j] != 0).sum()) == 0
+                continue
+            q = query[j].double().unflatten(0, (cache.num_heads, groups))
+            w = torch.einsum("hgd,lhd->hgl", q, kv[:seen] + kl[:seen]) * scale
+            size = torch.einsum("hgd,lhd->hgl", q.abs(), kv[:seen] + kl[:seen].abs()).amax(-1) * abs(scale) * math.log2(math.e)
+            p = torch.softmax(w, -1)
+            want = torch.einsum("hgl,lhd->hgd", p, vv[:seen] + vl[:seen])
+            mass = torch.einsum("hgl,lhd->hgd", p, vv[:seen] + vl[:seen].abs())
+            largest = torch.einsum("hgl,lhd->hgld", p, vv[:seen]).amax(2)
+            bound = want.abs() * (info.eps / 2) + (2.0 ** -11 + 2.0 ** -15 * size[..., None]) * mass \
+                + seen * 2.0 ** -20 * largest + info.smallest_normal
+            off = (got[j].double().unflatten(0, (cache.num_heads, groups)) - want).abs()
+            worst = max(worst, float((off / bound).max()))
+    assert worst <= 1, worst
+
+
+CASES = [
+    # lens, block, heads, kv_heads, head, dtype, tokens per sequence
+    ([1], 16, 32, 8, 128, torch.bfloat16, None),
+    ([0, 1, 31, 32, 33, 0], 16, 8, 2, 128, torch.float16, None),
+    ([1000], 16, 8, 1, 64, torch.bfloat16, None),
+    ([257, 5, 4100, 63], 24, 28, 4, 128, torch.bfloat16, None),      # groups of 7, pages that end inside a tile
+    ([700, 64], 1, 5, 5, 64, torch.float16, None),                   # one head a group, pages of one row
+    ([2049, 100], 64, 64, 2, 128, torch.bfloat16, None),             # groups of 32: row blocks of 16
+    ([40000], 128, 16, 2, 128, torch.bfloat16, None),
+    ([300, 9, 2, 1200], 16, 16, 4, 128, torch.bfloat16, [3, 1, 5, 4]),   # more tokens than keys in one
+    ([90, 0, 513], 24, 12, 4, 64, torch.float16, [17, 2, 40]),
+    ([3, 60], 7, 96, 2, 128, torch.float16, [1, 2]),
+]
+
+
+@pytest.mark.parametrize("case", CASES, ids=str)
+def test_against_64_bits(cuda, case):
+    lens, block, heads, kv_heads, head, dtype, counts = case
+    cache, table = _pages(cuda, lens, block, kv_heads, head, 3)
+    gen = torch.Generator(device=cuda).manual_seed(4)
+    start = None if counts is None else [0, *torch.tensor(counts).cumsum(0).tolist()]
+    total = len(lens) if counts is None else start[-1]
+    query = torch.randn(total, heads, head, generator=gen, device=cuda).to(dtype)
+    lengths = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    begin = None if start is None else torch.tensor(start, dtype=torch.int32, device=cuda)
+    got = paged_attention4(query, cache, table, lengths, head ** -0.5, query_start=begin)
+    _check(got, query, cache, table, lens, head ** -0.5, start)
+    again = paged_attention4(query, cache, table, lengths, head ** -0.5, query_start=begin)
+    assert torch.equal(got, again)
+
+
+@pytest.mark.parametrize("step,low,q", [((1e-4, 3e-4), (-1e-3, 1e-3), 1.0), ((40.0, 900.0), (-8000.0, 100.0), 1e-4),
+                                        ((0.0, 0.0), (-1.0, 1.0), 1.0), ((0.1, 0.2), (-1.0, 0.0), 30.0)])
+def test_sizes_of_values(cuda, step, low, q):
+    """Small, large and constant rows, and peaked logits."""
+    lens = [1500, 40]
+    cache, table = _pages(cuda, lens, 16, 2, 128, 5, step, low)
+    query = (torch.randn(2, 8, 128, device=cuda, generator=torch.Generator(device=cuda).manual_seed(6)) * q).to(torch.bfloat16)
+    got = paged_attention4(query, cache, table, torch.tensor(lens, dtype=torch.int32, device=cuda), 0.09)
+    _check(got, query, cache, table, lens, 0.09)
+
+
+def test_strides_rows_behind_and_bad_pages(cuda):
+    lens, heads, head = [200, 77], 8, 128
+    cache, table = _pages(cuda, lens, 16, 4, head, 7)
+    wide = torch.randn(6, heads + 3, head + 1, device=cuda, generator=torch.Generator(device=cuda).manual_seed(8)).to(torch.bfloat16)
+    query = wide[:, 1:1 + heads, 1:]  # rows that are not 16-byte aligned
+    start = torch.tensor([1, 2, 4], dtype=torch.int32, device=cuda)
+    lengths = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    out = torch.full((6, heads, head + 2), 5.0, device=cuda, dtype=torch.bfloat16)[..., 1:1 + head]
+    got = paged_attention4(query, cache, table, lengths, head ** -0.5, query_start=start, out=out)
+    assert got is out
+    _check(got, query, cache, table, lens, head ** -0.5, [1, 2, 4])
+    assert (got[0] == 5).all() and (got[4:] == 5).all()  # rows of no sequence
+    # a page outside the cache is left out: the same as a sequence without its keys
+    short = table.clone()
+    short[0, -(-lens[0] // 16) - 1] = cache.num_blocks + 4
+    cut = paged_attention4(query, cache, short, lengths, head ** -0.5, query_start=start)
+    fewer = torch.tensor([192, 77], dtype=torch.int32, device=cuda)
+    assert torch.equal(cut[2:4], got[2:4])
+    same = paged_attention4(query, cache, table, fewer, head ** -0.5, query_start=start)
+    assert torch.equal(cut[1], same[1])
+    # lengths past the table, starts past the rows: clamped
+    over = paged_attention4(query, cache, table[:, :5].contiguous(), torch.tensor([10 ** 6, 77], dtype=torch.int32, device=cuda),
+                            head ** -0.5, query_start=torch.tensor([1, 2, 99], dtype=torch.int32, device=cuda))
+    want = paged_attention4(query, cache, table, torch.tensor([80, 77], dtype=torch.int32, device=cuda), head ** -0.5,
+                            query_start=torch.tensor([1, 2, 6], dtype=torch.int32, device=cuda))
+    assert torch.equal(over[1:], want[1:])
+
+
+def test_not_finite(cuda):
+    """A NaN row reaches the tokens that see it and no other."""
+    lens = [100]
+    for plane in (0, 1):
+        cache, table = _pages(cuda, lens, 16, 1, 64, 9)
+        cache.scales[plane, table[0, 6], 0, 2, 0, 0] = torch.nan  # key 98
+        query = torch.randn(3, 2, 64, device=cuda, generator=torch.Generator(device=cuda).manual_seed(1)).to(torch.float16)
+        got = paged_attention4(query, cache, table, torch.tensor(lens, dtype=torch.int32, device=cuda), 0.125,
+                               query_start=torch.tensor([0, 3], dtype=torch.int32, device=cuda))
+        assert bool(got[0].isfinite().all()) and bool(got[1:].isnan().all())
+    cache, table = _pages(cuda, [100, 50], 16, 1, 64, 9)
+    query[0, 1] = torch.inf  # a bad query head keeps to itself
+    got = paged_attention4(query[:2], cache, table, torch.tensor([100, 50], dtype=torch.int32, device=cuda), 0.125)
+    assert bool(got[0, 1].isnan().all()) and bool(got[0, 0].isfinite().all()) and bool(got[1].isfinite().all())
+
+
+def test_many_sequences(cuda):
+    """More sequences than threads of a CTA, most of them empty or short."""
+    gen = torch.Generator().manual_seed(10)
+    lens = (torch.rand(700, generator=gen) ** 4 * 300).long().tolist()
+    cache, table = _pages(cuda, lens, 16, 2, 64, 11)
+    query = torch.randn(700, 4, 64, device=cuda, generator=torch.Generator(device=cuda).manual_seed(1)).to(torch.bfloat16)
+    got = paged_attention4(query, cache, table, torch.tensor(lens, dtype=torch.int32, device=cuda), 0.125)
+    _check(got, query, cache, table, lens, 0.125)
+
+
+def test_offsets_past_32_bits(cuda):
+    """Pages that lie past a 32-bit byte offset of the codes."""
+    block, kv_heads, head = 128, 8, 128
+    blocks = (1 << 32) // (block * kv_heads * head // 2) + 30
+    codes = torch.empty(2, blocks, kv_heads, block, head // 2, dtype=torch.uint8, device=cuda)
+    scales = torch.zeros(2, blocks, kv_heads, block, 2, 2, dtype=torch.float16, device=cuda)
+    small, table = _pages(cuda, [500, 130], block, kv_heads, head, 12)
+    moved = torch.where(table >= 0, table + blocks - small.num_blocks, table)
+    codes[:, -small.num_blocks:], scales[:, -small.num_blocks:] = small.codes, small.scales
+    query = torch.randn(2, 32, head, device=cuda, generator=torch.Generator(device=cuda).manual_seed(1)).to(torch.bfloat16)
+    lengths = torch.tensor([500, 130], dtype=torch.int32, device=cuda)
+    want = paged_attention4(query, small, table, lengths, head ** -0.5)
+    assert torch.equal(paged_attention4(query, PagedKV4(codes, scales), moved, lengths, head ** -0.5), want)
+
+
+def test_streams_workspace_and_graph(cuda):
+    lens = [900, 33]
+    cache, table = _pages(cuda, lens, 16, 2, 128, 13)
+    query = torch.randn(2, 8, 128, device=cuda, generator=torch.Generator(device=cuda).manual_seed(1)).to(torch.bfloat16)
+    lengths = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    want = paged_attention4(query, cache, table, lengths, 0.1)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream(cuda)
+    got = paged_attention4(query, cache, table, lengths, 0.1, stream=side)
+    side.synchronize()
+    assert torch.equal(got, want)
+    size = paged_attention4_workspace_bytes(2, 2, 8, 2, 128)
+    dirty = torch.full((size,), 255, dtype=torch.uint8, device=cuda)
+    assert torch.equal(paged_attention4(query, cache, table, lengths, 0.1, workspace=dirty), want)
+    with pytest.raises(ValueError, match="workspace"):
+        paged_attention4(query, cache, table, lengths, 0.1, workspace=dirty[:size - 16])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        inside = paged_attention4(query, cache, table, lengths, 0.1)
+    lengths.copy_(torch.tensor([300, 20], dtype=torch.int32))  # the next step's lengths
+    graph.replay()
+    torch.cuda.synchronize()
+    _check(inside, query, cache, table, [300, 20], 0.1)
+
+
+def test_append_then_attend(cuda):
+    """A prompt and decode steps through the pages, as a serving loop makes them."""
+    block, kv_heads, heads, head = 16, 2, 8, 128
+    gen = torch.Generator(device=cuda).manual_seed(20)
+    cache = PagedKV4.allocate(12, block, kv_heads, head, cuda)
+    table = torch.tensor([[3, 0, 7, 9], [1, 11, 2, 4]], dtype=torch.int32, device=cuda)
+    lens = torch.tensor([30, 7], dtype=torch.int32, device=cuda)
+
+    def fresh(n):
+        return (torch.randn(n, kv_heads, head, generator=gen, device=cuda).to(torch.bfloat16) for _ in range(2))
+
+    for i, n in enumerate(lens.tolist()):
+        k, v = fresh(n)
+        at = torch.arange(n, device=cuda)
+        append_paged_kv4(None, None, k, v, cache, table[i, at // block].long() * block + at % block)
+    for _ in range(4):
+        k, v = fresh(2)
+        at = lens.long()
+        append_paged_kv4(None, None, k, v, cache, table[torch.arange(2, device=cuda), at // block].long() * block + at % block)
+        lens += 1
+        query = torch.randn(2, heads, head, generator=gen, device=cuda).to(torch.bfloat16)
+        got = paged_attention4(query, cache, table, lens, head ** -0.5)
+        _check(got, query, cache, table, lens.tolist(), head ** -0.5)
+    assert gather_paged_kv4(cache, table[0, :1].long() * block).isfinite().all()
