@@ -100,7 +100,7 @@ CASES = [
     ([1000], 16, 8, 1, 64, torch.bfloat16, None),
     ([257, 5, 4100, 63], 24, 28, 4, 128, torch.bfloat16, None),      # groups of 7, pages that end inside a tile
     ([700, 64], 1, 5, 5, 64, torch.float16, None),                   # one head a group, pages of one row
-    ([2049, 100], 64, 64, 2, 128, torch.bfloat16, None),             # groups of 32: row blocks of 16
+    ([2049, 100], 64, 64, 2, 128, torch.bfloat16, None),             # groups of 32: four row blocks
     ([40000], 128, 16, 2, 128, torch.bfloat16, None),
     ([300, 9, 2, 1200], 16, 16, 4, 128, torch.bfloat16, [3, 1, 5, 4]),   # more tokens than keys in one
     ([90, 0, 513], 24, 12, 4, 64, torch.float16, [17, 2, 40]),
