@@ -528,6 +528,37 @@ CB_API int cb_paged_attention4(const void* query, int64_t query_token_stride,
                                int64_t out_head_stride, void* workspace, int64_t workspace_bytes,
                                void* stream);
 
+/*
+ * Causal attention of a packed batch of prompts: sequence i owns the query rows
+ * query_start[i] .. query_start[i + 1] - 1 and the key rows key_start[i] ..
+ * key_start[i + 1] - 1 (device int32 [num_seqs + 1], ascending; the same array
+ * where nothing is cached); its n queries are the last n of its k keys, query j
+ * sees the keys at or before k - n + j.  query, out: [num_queries][num_q_heads]
+ * [head_size], key, value: [num_keys][num_kv_heads][head_size], bf16 or fp16,
+ * heads of 64 or 128 values, at most 128 query heads to a KV head, token and
+ * head strides in bytes, rows 16-byte aligned; scale > 0.  Logits, softmax and
+ * sums in fp32, the probabilities rounded to the element type for the second
+ * product.  A query that sees no key gives zeros; rows of no sequence are not
+ * written; starts are clamped to the rows there are.  What a masked place holds
+ * (NaN, infinities) reaches no output.  `workspace`: 16-byte aligned device
+ * memory of cb_prompt_attention_workspace_size bytes, any contents; calls that
+ * share one must not overlap on the GPU.  On the tensor cores (tcgen05.mma, TMA);
+ * device_error (optional) receives a code if a bounded wait gives up.
+ */
+CB_API int cb_prompt_attention_workspace_size(int64_t num_queries, int64_t num_seqs,
+                                              int64_t num_q_heads, int64_t num_kv_heads,
+                                              int64_t head_size, int64_t* bytes);
+CB_API int cb_prompt_attention(const void* query, int64_t query_token_stride,
+                               int64_t query_head_stride, const void* key, int64_t key_token_stride,
+                               int64_t key_head_stride, const void* value,
+                               int64_t value_token_stride, int64_t value_head_stride,
+                               int64_t num_queries, int64_t num_keys, int64_t num_q_heads,
+                               int64_t num_kv_heads, int64_t head_size, int dtype,
+                               const int32_t* query_start, const int32_t* key_start,
+                               int64_t num_seqs, float scale, void* out, int64_t out_token_stride,
+                               int64_t out_head_stride, void* workspace, int64_t workspace_bytes,
+                               int32_t* device_error, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,7 +8,7 @@ mirrors of the reference types: ``CacheBlendConfig``, ``BlendPlan``,
 """
 
 from .append import PagedKV4, append_paged_kv, append_paged_kv4, gather_paged_kv4
-from .attention import paged_attention4
+from .attention import paged_attention4, prompt_attention
 from .config import CacheBlendConfig
 from .kv_layout import gather_paged_kv, scatter_paged_kv
 from .loader import PagedBlendLoader
@@ -33,6 +33,7 @@ __all__ = [
     "gather_paged_kv4",
     "kv_deviation",
     "paged_attention4",
+    "prompt_attention",
     "recompute_budget",
     "relocate_key",
     "scatter_paged_kv",

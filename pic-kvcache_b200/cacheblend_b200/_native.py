@@ -158,6 +158,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          _i64, _i64, _i64, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, ctypes.c_float, _ptr, _i64,
          _i64, _ptr, _i64, _ptr],
     ),
+    "cb_prompt_attention_workspace_size": (_i32, [_i64, _i64, _i64, _i64, _i64, _ptr]),
+    "cb_prompt_attention": (
+        _i32,
+        [_ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32,
+         _ptr, _ptr, _i64, ctypes.c_float, _ptr, _i64, _i64, _ptr, _i64, _ptr, _ptr],
+    ),
 }
 
 _lock = threading.Lock()

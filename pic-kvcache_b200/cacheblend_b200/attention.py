@@ -1,10 +1,10 @@
-"""Attention: of a blend request's staging, and of decode steps over 4-bit pages.
+"""Attention: of a blend request's staging, of packed prompts, and of decode steps over 4-bit pages.
 
 Blend attention on the tensor cores (cb_blend_attention): the side executor's attention of the computed, possibly pruned, queries over
 the whole staging context: Qwen3BlendExecutor._attention
 (cacheblend_vllm/ascend.py:798-846).  Queries sit at absolute positions and
 attend every staging row at or before their position; grouped query heads
-share their KV head.  ``paged_attention4``: at the end of the file.
+share their KV head.  ``prompt_attention`` and ``paged_attention4``: at the end of the file.
 """
 
 from __future__ import annotations
@@ -191,4 +191,93 @@ def paged_attention4(
             cache.num_blocks, cache.block_size, cache.num_heads, head_size,
             block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), seqs, float(scale),
             result.data_ptr(), 2 * out_token, 2 * out_row, workspace.data_ptr(), workspace.numel(), current_handle())
+        return result
+
+
+def prompt_attention_workspace_bytes(num_queries: int, num_seqs: int, num_q_heads: int, num_kv_heads: int,
+                                     head_size: int) -> int:
+    size = ctypes.c_int64(0)
+    _native.call("cb_prompt_attention_workspace_size", num_queries, num_seqs, num_q_heads, num_kv_heads, head_size,
+                 ctypes.addressof(size))
+    return int(size.value)
+
+
+def prompt_attention(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    query_start: torch.Tensor,
+    scale: float,
+    key_start: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+    device_error: torch.Tensor | None = None,
+    stream: torch.cuda.Stream | None = None,
+) -> torch.Tensor:
+    """Causal attention of a packed batch of prompts: ``[tokens, q_heads, head_size]``.
+
+    ``query``: ``[tokens, q_heads, head_size]``, ``key`` and ``value``: ``[keys, kv_heads, head_size]``,
+    bf16 or fp16, heads of 64 or 128 values, rows 16-byte aligned (slices of one projection's
+    output will do); query head h attends KV head ``h // (q_heads // kv_heads)``.
+    ``query_start``: int32 ``[seqs + 1]`` on the device, where each sequence's rows begin,
+    ascending; ``key_start`` the same for its keys, if it has more of them than queries (a
+    cached prefix): its n queries are then the last n of its k keys, and query j sees the keys
+    at or before ``k - n + j``.
+
+    A query that sees no key gives zeros; rows of no sequence are left as ``out`` held them, and
+    nothing that a masked place or another sequence holds reaches an output.  ``scale`` must be
+    positive.  ``workspace``: ``prompt_attention_workspace_bytes`` of uint8, for callers that keep
+    one (two calls that may overlap need two); otherwise allocated per call.
+    """
+    if query.ndim != 3 or key.ndim != 3 or value.shape != key.shape:
+        raise ValueError("query must be [tokens, q_heads, head_size]; key and value [keys, kv_heads, head_size]")
+    if query.dtype not in (torch.bfloat16, torch.float16):
+        raise NotImplementedError(f"prompt attention needs bfloat16 or float16, not {query.dtype}")
+    if not (query.dtype == key.dtype == value.dtype):
+        raise ValueError("query, key and value must share a dtype")
+    tokens, heads, head_size = query.shape
+    keys, kv_heads, _ = key.shape
+    if key.shape[2] != head_size or kv_heads == 0 or heads == 0 or heads % kv_heads:
+        raise ValueError(f"query {tuple(query.shape)} does not fit keys {tuple(key.shape)}")
+    device = query.device
+    if key.device != device or value.device != device:
+        raise ValueError("query, key and value must live on one device")
+    for name, t in (("query", query), ("key", key), ("value", value)):
+        if t.stride(2) != 1:
+            raise ValueError(f"{name} heads must be contiguous")
+    _int32("query_start", query_start, device, 1)
+    if query_start.shape[0] == 0:
+        raise ValueError("query_start must hold one entry per sequence and one more")
+    if key_start is None:
+        if keys != tokens:
+            raise ValueError(f"{keys} keys for {tokens} queries need key_start")
+        key_start = query_start
+    else:
+        _int32("key_start", key_start, device, 1)
+        if key_start.shape[0] != query_start.shape[0]:
+            raise ValueError("key_start must hold as many entries as query_start")
+    if not scale > 0:
+        raise ValueError(f"the scale must be positive, not {scale}")
+    if device_error is not None and (device_error.dtype != torch.int32 or device_error.device != device):
+        raise ValueError("device_error must be int32 on the query's device")
+    _native.require_cuda(query)
+    seqs = query_start.shape[0] - 1
+    with on_device(device, stream):
+        result = _attention_out(query, out)
+        if tokens == 0 or seqs == 0:
+            return result
+        if keys == 0:
+            raise ValueError("prompt attention needs keys")
+        need = prompt_attention_workspace_bytes(tokens, seqs, heads, kv_heads, head_size)
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        elif workspace.dtype != torch.uint8 or workspace.device != device or not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous uint8 on the query's device")
+        strides = [2 * s for t in (query, key, value, result) for s in t.stride()[:2]]
+        _native.call(
+            "cb_prompt_attention", query.data_ptr(), strides[0], strides[1], key.data_ptr(), strides[2], strides[3],
+            value.data_ptr(), strides[4], strides[5], tokens, keys, heads, kv_heads, head_size,
+            _native.DTYPE_CODES[query.dtype], query_start.data_ptr(), key_start.data_ptr(), seqs, float(scale),
+            result.data_ptr(), strides[6], strides[7], workspace.data_ptr(), workspace.numel(),
+            0 if device_error is None else device_error.data_ptr(), current_handle())
         return result
