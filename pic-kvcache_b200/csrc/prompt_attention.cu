@@ -145,6 +145,15 @@ __device__ __forceinline__ bool finite2(uint32_t w) {
   return (w & kExp) != kExp && ((w >> 16) & kExp) != kExp;
 }
 
+// 32 lanes x 16 consecutive columns of this warp's TMEM sub-partition, stored.
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(addr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
 template <typename T, int N>
 __host__ __device__ constexpr uint32_t instr_desc() {
   constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
@@ -451,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float m_new = grow ? tile_max : m_used;
           const float corr = grow ? (m_used == -INFINITY ? 0.0f : ex2(m_used - m_new)) : 1.0f;
           if (kt > 0) {  // O holds earlier tiles of this item, all finished: rescale its rows
-#pragma unroll
+#pragma unroll 1
             for (int q = 0; q < D / 32; ++q) {
               uint32_t o[32];
               tmem_ld32(o_tmem + q * 32, o);
@@ -472,21 +481,23 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) sm[i] = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {  // P of 64 keys: 32 columns over the S that was read
-          uint32_t packed[32];
+        for (int part = 0; part < 4; ++part) {  // P of 32 keys: 16 columns over the S that was read
+          uint32_t packed[16];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float2 s2 = make_float2(s_of(half * 64 + 2 * j), s_of(half * 64 + 2 * j + 1));
+          for (int j = 0; j < 16; ++j) {
+            const float2 s2 = make_float2(s_of(part * 32 + 2 * j), s_of(part * 32 + 2 * j + 1));
             const float2 e2 = __ffma2_rn(s2, mul, nm);
             const float2 p2 = make_float2(ex2(e2.x), ex2(e2.y));
             sm[j & 3] = __fadd2_rn(sm[j & 3], p2);
             packed[j] = pack2<T>(p2.x, p2.y);
           }
-          tmem_st32(s_tmem + half * 32, packed);
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.p_full[x][half]);
+          tmem_st16(s_tmem + part * 16, packed);
+          if (part & 1) {  // 64 keys: the first of the product's two halves, or the second
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.p_full[x][part >> 1]);
+          }
         }
         const float2 st = __fadd2_rn(__fadd2_rn(sm[0], sm[1]), __fadd2_rn(sm[2], sm[3]));
         l += st.x + st.y;
@@ -503,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool odd = *reinterpret_cast<volatile int*>(&sh.odd_values) != 0;
       const bool seen = n > 0 && pos >= 0;
       const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-#pragma unroll
+#pragma unroll 1
       for (int q = 0; q < D / 32; ++q) {
         uint32_t o[32];
         if (n > 0) {
