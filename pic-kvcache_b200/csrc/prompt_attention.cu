@@ -51,8 +51,8 @@ namespace prompt {
 using namespace ::cb::tc;
 
 constexpr int kPair = 2;     // query tiles per item, one softmax warpgroup each
-constexpr int kKStages = 3;
-constexpr int kVStages = 2;
+constexpr int kKStages = 2;
+constexpr int kVStages = 3;
 constexpr int kThreads = 384;
 constexpr uint32_t kTmemCols = 512;  // S_A [0,128) S_B [128,256) O_A [256,384) O_B [384,512)
 constexpr uint32_t kTmemO = 256;
@@ -347,68 +347,65 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr uint32_t kDescPV = instr_desc<T, D>() | (1u << 16);  // B (V) MN-major
         const uint32_t q_addr = smem_u32(q_buf), k_addr = smem_u32(k_buf), v_addr = smem_u32(v_buf);
         const uint32_t tmem = sh.tmem_base;
-        int kt_all = 0, vt_all = 0, it = 0;  // K and V tiles and items so far
+        int it = 0;                                // items so far
+        int ks = 0, vs = 0;                        // ring slots and their parities: running, since the
+        uint32_t kp = 0, vp = 0;                   // divisions would stand between two products
         int p_count[kPair] = {0, 0}, o_count[kPair] = {0, 0};
         bool ok = true;
+        auto issue_s = [&](int x) {
+#pragma unroll
+          for (int i = 0; i < kHalves; ++i)
+            product_s(tmem + x * kTile, desc_lo(q_addr + x * kBytes + i * kHalfBytes),
+                      desc_lo(k_addr + ks * kBytes + i * kHalfBytes), kDescS, i > 0);
+          umma_commit(&sh.s_full[x]);
+        };
+        auto next_k = [&]() {
+          if (++ks == kKStages) ks = 0, kp ^= 1;
+        };
         for (int k = 0, item = cta_item(0); item < items && ok && !aborted(sh); item = cta_item(++k)) {
           const Item w = load_item(c, item);
           const int n[kPair] = {tile_count(c, w, 0), tile_count(c, w, 1)};
           const int tiles = max(n[0], n[1]);
           if (tiles == 0) continue;
-          if (!wait1(&sh.q_full, it & 1)) { ok = false; break; }
+          if (!wait1(&sh.q_full, it & 1) || !wait1(&sh.k_full[ks], kp)) { ok = false; break; }
           ++it;
-          auto issue_s = [&](int x, int kt) {  // K tile kt of the item has been waited for
-            const int s = (kt_all + kt) % kKStages;
-            for (int i = 0; i < kHalves; ++i)
-              product_s(tmem + x * kTile, desc_lo(q_addr + x * kBytes + i * kHalfBytes),
-                        desc_lo(k_addr + s * kBytes + i * kHalfBytes), kDescS, i > 0);
-            umma_commit(&sh.s_full[x]);
-          };
-          auto wait_k = [&](int kt) { return wait1(&sh.k_full[(kt_all + kt) % kKStages], ((kt_all + kt) / kKStages) & 1); };
-          auto free_k = [&](int kt) {
-            umma_commit(&sh.k_empty[(kt_all + kt) % kKStages]);
-            if (kt + 1 == tiles) umma_commit(&sh.q_empty);  // every S of this item is issued
-          };
-          if (!wait_k(0)) { ok = false; break; }
           tc_fence_after();
 #pragma unroll
           for (int x = 0; x < kPair; ++x)
-            if (n[x] > 0) issue_s(x, 0);
-          free_k(0);
-          for (int kt = 0; kt < tiles && ok; ++kt) {
-            const int vs = (vt_all + kt) % kVStages;
+            if (n[x] > 0) issue_s(x);
+          next_k();
+          for (int kt = 0; kt < tiles; ++kt) {
+            ok = wait1(&sh.v_full[vs], vp);
             const uint32_t v_rows = v_addr + vs * kBytes;
-            bool next_k = false;
+            bool have_k = kt + 1 >= tiles;
 #pragma unroll
             for (int x = 0; x < kPair; ++x) {
-              if (kt >= n[x]) continue;
-              if (!wait1(&sh.v_full[vs], ((vt_all + kt) / kVStages) & 1)) { ok = false; break; }
-              if (kt == 0 && !wait1(&sh.o_empty[x], (o_count[x] & 1) ^ 1)) { ok = false; break; }
-#pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                if (!wait1(&sh.p_full[x][half], p_count[x] & 1)) { ok = false; break; }
-                tc_fence_after();
-                product_pv(tmem + kTmemO + x * kTile, tmem + x * kTile + half * 32, desc_lo_mn(v_rows + half * 64 * 128), kDescPV,
-                           kt > 0 || half > 0);
-              }
+              if (kt >= n[x] || !ok) continue;
+              const uint32_t parity = p_count[x] & 1;
+              if (kt == 0) ok = wait1(&sh.o_empty[x], (o_count[x] & 1) ^ 1);
+              ok = ok && wait1(&sh.p_full[x][0], parity);
               if (!ok) break;
+              tc_fence_after();
+              product_pv(tmem + kTmemO + x * kTile, tmem + x * kTile, desc_lo_mn(v_rows), kDescPV, kt > 0);
+              // the next K's barrier is looked at while the tensor cores have half of P V to do
+              if (!have_k) ok = wait1(&sh.k_full[ks], kp);
+              have_k = true;
+              ok = ok && wait1(&sh.p_full[x][1], parity);
+              if (!ok) break;
+              tc_fence_after();
+              product_pv(tmem + kTmemO + x * kTile, tmem + x * kTile + 32, desc_lo_mn(v_rows + 64 * 128), kDescPV, true);
               ++p_count[x];
-              if (x == 1 || kt >= n[1]) umma_commit(&sh.v_empty[vs]);  // the tile's last use
-              if (kt + 1 == n[x]) {
+              if (kt + 1 < n[x]) {
+                issue_s(x);
+              } else {
                 umma_commit(&sh.o_full[x]);
                 ++o_count[x];
               }
-              if (kt + 1 < n[x]) {
-                if (!next_k && !wait_k(kt + 1)) { ok = false; break; }
-                next_k = true;
-                tc_fence_after();
-                issue_s(x, kt + 1);
-              }
             }
-            if (ok && next_k) free_k(kt + 1);
+            if (!ok) break;
+            if (++vs == kVStages) vs = 0, vp ^= 1;
+            if (kt + 1 < tiles) next_k();
           }
-          kt_all += tiles;
-          vt_all += tiles;
         }
         if (!ok) report(c, sh, 2);
         umma_commit(&sh.drain);
@@ -425,18 +422,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_tmem = sh.tmem_base + x * kTile + lane_off;
     const uint32_t o_tmem = sh.tmem_base + kTmemO + x * kTile + lane_off;
     const int query_in_tile = row_in_tile / c.groups, group = row_in_tile - query_in_tile * c.groups;
-    int t = 0, o_count = 0;
+    // This warpgroup gives back what its products were the last to read: K of a tile (and Q with the
+    // item's last) once its S is there, V once the next S, or O, is.  The MMA thread would need a
+    // commit for each, and a commit behind a commit holds it up until the first has arrived (470
+    // cycles of a tile pair's 3,600).
+    const bool keeper = ew == 0 && lane == 0;
+    int t = 0, o_count = 0, tiles_before = 0;
     bool ok = true;
     for (int k = 0, item = cta_item(0); item < items && ok; item = cta_item(++k)) {
       const Item w = load_item(c, item);
       const int h = item % c.kv_heads;
-      const int n = tile_count(c, w, x);
+      const int n = tile_count(c, w, x), n_b = tile_count(c, w, 1);
+      auto last_reader = [&](int kt) { return x == 1 || kt >= n_b; };
       const bool store = query_in_tile < tile_valid(c, w, x);
       const int pos = w.pos + x * c.tile_queries + query_in_tile;  // the last key this row sees
       float m_used = -INFINITY;  // log2-domain maximum the exponentials are taken against
       float l = 0.0f;
       for (int kt = 0; kt < n; ++kt, ++t) {
         if (!wait_warp(&sh.s_full[x], t & 1)) { ok = false; break; }
+        if (keeper) {
+          if (last_reader(kt)) mbar_arrive(&sh.k_empty[(tiles_before + kt) % kKStages]);
+          if (kt > 0 && last_reader(kt - 1)) mbar_arrive(&sh.v_empty[(tiles_before + kt - 1) % kVStages]);
+          if (kt + 1 == n && last_reader(kt)) mbar_arrive(&sh.q_empty);
+        }
         tc_fence_after();
         uint32_t v[4][32];
 #pragma unroll
@@ -508,8 +516,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (n > 0) {
         if (!wait_warp(&sh.o_full[x], o_count & 1)) { ok = false; break; }
         ++o_count;
+        if (keeper && last_reader(n - 1)) mbar_arrive(&sh.v_empty[(tiles_before + n - 1) % kVStages]);
         tc_fence_after();
       }
+      tiles_before += max(n, tile_count(c, w, x ^ 1));
       // the P V of the item's boundary tiles came after their look-through
       const bool odd = *reinterpret_cast<volatile int*>(&sh.odd_values) != 0;
       const bool seen = n > 0 && pos >= 0;
