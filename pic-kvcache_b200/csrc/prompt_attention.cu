@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int it = 0;                                // items so far
         int ks = 0, vs = 0;                        // ring slots and their parities: running, since the
         uint32_t kp = 0, vp = 0;                   // divisions would stand between two products
-        int p_count[kPair] = {0, 0}, o_count[kPair] = {0, 0};
+        uint32_t pp[kPair] = {0, 0}, op[kPair] = {1, 1};  // parities of P and of O's release
         bool ok = true;
         auto issue_s = [&](int x) {
 #pragma unroll
@@ -358,6 +358,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             product_s(tmem + x * kTile, desc_lo(q_addr + x * kBytes + i * kHalfBytes),
                       desc_lo(k_addr + ks * kBytes + i * kHalfBytes), kDescS, i > 0);
           umma_commit(&sh.s_full[x]);
+        };
+        auto issue_pv = [&](int x, int half, uint32_t v_rows, bool onto) {
+          tc_fence_after();
+          product_pv(tmem + kTmemO + x * kTile, tmem + x * kTile + half * 32, desc_lo_mn(v_rows + half * 64 * 128), kDescPV,
+                     onto);
         };
         auto next_k = [&]() {
           if (++ks == kKStages) ks = 0, kp ^= 1;
@@ -374,37 +379,57 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int x = 0; x < kPair; ++x)
             if (n[x] > 0) issue_s(x);
           next_k();
-          for (int kt = 0; kt < tiles; ++kt) {
-            ok = wait1(&sh.v_full[vs], vp);
+          ok = wait1(&sh.v_full[vs], vp);  // (V of each next tile is looked for behind P V)
+#pragma unroll
+          for (int x = 0; x < kPair; ++x)
+            if (n[x] > 0) ok = wait1(&sh.o_empty[x], op[x]) && ok, op[x] ^= 1;
+          int kt = 0;
+          // Tiles that both query tiles have a successor of.  Every look at a barrier stands where the
+          // products issued before it still have time to run (the issue of a product waits for the
+          // third before it, so 200 cycles); a wait that ran out is acted on at the end of the round.
+          for (; ok && kt + 1 < min(n[0], n[1]); ++kt) {
+            const uint32_t v_rows = v_addr + vs * kBytes;
+            const bool onto = kt > 0;
+            ok = wait1(&sh.p_full[0][0], pp[0]);
+            issue_pv(0, 0, v_rows, onto);
+            ok = wait1(&sh.k_full[ks], kp) && ok;
+            ok = wait1(&sh.p_full[0][1], pp[0]) && ok;
+            issue_pv(0, 1, v_rows, true);
+            issue_s(0);
+            ok = wait1(&sh.p_full[1][0], pp[1]) && ok;
+            issue_pv(1, 0, v_rows, onto);
+            ok = wait1(&sh.p_full[1][1], pp[1]) && ok;
+            issue_pv(1, 1, v_rows, true);
+            if (++vs == kVStages) vs = 0, vp ^= 1;
+            ok = wait1(&sh.v_full[vs], vp) && ok;
+            issue_s(1);
+            next_k();
+            pp[0] ^= 1, pp[1] ^= 1;
+          }
+          // the last tiles of either
+          for (; ok && kt < tiles; ++kt) {
             const uint32_t v_rows = v_addr + vs * kBytes;
             bool have_k = kt + 1 >= tiles;
 #pragma unroll
             for (int x = 0; x < kPair; ++x) {
-              if (kt >= n[x] || !ok) continue;
-              const uint32_t parity = p_count[x] & 1;
-              if (kt == 0) ok = wait1(&sh.o_empty[x], (o_count[x] & 1) ^ 1);
-              ok = ok && wait1(&sh.p_full[x][0], parity);
-              if (!ok) break;
-              tc_fence_after();
-              product_pv(tmem + kTmemO + x * kTile, tmem + x * kTile, desc_lo_mn(v_rows), kDescPV, kt > 0);
-              // the next K's barrier is looked at while the tensor cores have half of P V to do
-              if (!have_k) ok = wait1(&sh.k_full[ks], kp);
+              if (kt >= n[x]) continue;
+              ok = wait1(&sh.p_full[x][0], pp[x]) && ok;
+              issue_pv(x, 0, v_rows, kt > 0);
+              if (!have_k) ok = wait1(&sh.k_full[ks], kp) && ok;
               have_k = true;
-              ok = ok && wait1(&sh.p_full[x][1], parity);
-              if (!ok) break;
-              tc_fence_after();
-              product_pv(tmem + kTmemO + x * kTile, tmem + x * kTile + 32, desc_lo_mn(v_rows + 64 * 128), kDescPV, true);
-              ++p_count[x];
-              if (kt + 1 < n[x]) {
+              ok = wait1(&sh.p_full[x][1], pp[x]) && ok;
+              issue_pv(x, 1, v_rows, true);
+              pp[x] ^= 1;
+              if (kt + 1 < n[x])
                 issue_s(x);
-              } else {
+              else
                 umma_commit(&sh.o_full[x]);
-                ++o_count[x];
-              }
             }
-            if (!ok) break;
             if (++vs == kVStages) vs = 0, vp ^= 1;
-            if (kt + 1 < tiles) next_k();
+            if (kt + 1 < tiles) {
+              next_k();
+              ok = ok && wait1(&sh.v_full[vs], vp);
+            }
           }
         }
         if (!ok) report(c, sh, 2);
@@ -438,8 +463,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int pos = w.pos + x * c.tile_queries + query_in_tile;  // the last key this row sees
       float m_used = -INFINITY;  // log2-domain maximum the exponentials are taken against
       float l = 0.0f;
-      for (int kt = 0; kt < n; ++kt, ++t) {
-        if (!wait_warp(&sh.s_full[x], t & 1)) { ok = false; break; }
+      // A tile of S; MASKED: some row of this warp does not see all of it.  Two copies, so that the
+      // loop that runs longest is short: with the masks' code in it, skipped, it ran 6 % slower.
+      auto softmax_tile = [&](auto masked_tag, int kt) {
+        constexpr bool MASKED = decltype(masked_tag)::value;
         if (keeper) {
           if (last_reader(kt)) mbar_arrive(&sh.k_empty[(tiles_before + kt) % kKStages]);
           if (kt > 0 && last_reader(kt - 1)) mbar_arrive(&sh.v_empty[(tiles_before + kt - 1) % kVStages]);
@@ -450,8 +477,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int q = 0; q < 4; ++q) tmem_ld32(s_tmem + q * 32, v[q]);
         tmem_wait_ld();
-        const int valid = min(max(pos - kt * kTile + 1, 0), kTile);
-        if (valid < kTile) {  // this row does not see the whole tile
+        if constexpr (MASKED) {
+          const int valid = min(max(pos - kt * kTile + 1, 0), kTile);
 #pragma unroll
           for (int j = 0; j < kTile; ++j)
             if (j >= valid) v[j >> 5][j & 31] = __float_as_uint(-INFINITY);
@@ -509,6 +536,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const float2 st = __fadd2_rn(__fadd2_rn(sm[0], sm[1]), __fadd2_rn(sm[2], sm[3]));
         l += st.x + st.y;
+      };
+      // whole tiles: up to the last key that the warp's first row sees
+      const int first_pos = w.pos + x * c.tile_queries + ew * 32 / c.groups;
+      const int whole = min(max(first_pos + 1, 0) / kTile, n);
+      int kt = 0;
+#pragma unroll 1
+      for (; kt < whole; ++kt, ++t) {
+        if (!wait_warp(&sh.s_full[x], t & 1)) { ok = false; break; }
+        softmax_tile(std::false_type{}, kt);
+      }
+#pragma unroll 1
+      for (; ok && kt < n; ++kt, ++t) {
+        if (!wait_warp(&sh.s_full[x], t & 1)) { ok = false; break; }
+        softmax_tile(std::true_type{}, kt);
       }
       if (!ok) break;
       T* dst = reinterpret_cast<T*>(c.out + (static_cast<int64_t>(w.q_row) + x * c.tile_queries + query_in_tile) * c.out_ts +
