@@ -138,13 +138,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// Whether the two elements of a word are finite.
-template <typename T>
-__device__ __forceinline__ bool finite2(uint32_t w) {
-  constexpr uint32_t kExp = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
-  return (w & kExp) != kExp && ((w >> 16) & kExp) != kExp;
-}
-
 // 32 lanes x 16 consecutive columns of this warp's TMEM sub-partition, stored.
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
   asm volatile(
@@ -283,26 +276,36 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ------------------------------------------------------ V loads, and a look at boundary tiles
       int t = 0, issued = 0;  // tiles so far, and of them the loads that are on their way or done
       bool ok = true;
+      constexpr uint32_t kExp2 = std::is_same<T, __nv_bfloat16>::value ? 0x7f807f80u : 0x7c007c00u;
+      constexpr uint32_t kOne2 = std::is_same<T, __nv_bfloat16>::value ? 0x00800080u : 0x04000400u;
       // hands tile u on once it has landed; `from`: its first key that some row does not see
       auto hand_on = [&](int u, int from) -> bool {
         const int s = u % kVStages;
         if (!wait_warp(&sh.v_landed[s], (u / kVStages) & 1)) return false;
         if (from < kTile) {
-          constexpr uint32_t kExp = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
-          uint4* rows = reinterpret_cast<uint4*>(v_buf + s * kBytes);
-          bool odd = false;
-          for (int i = lane; i < kBytes / 16; i += 32) {  // 8 vectors a row of a half
-            if (((i >> 3) & (kTile - 1)) < from) continue;
-            uint4 v = rows[i];
-            if (finite2<T>(v.x) && finite2<T>(v.y) && finite2<T>(v.z) && finite2<T>(v.w)) continue;
-            uint32_t* e = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              if ((e[j] & kExp) == kExp) e[j] &= 0xffff0000u;
-              if (((e[j] >> 16) & kExp) == kExp) e[j] &= 0xffffu;
+          // a lane looks at the same 16 bytes of every fourth row; an exponent of all ones carries
+          // into its element's sign bit
+          uint32_t carries = 0;
+          for (int half = 0; half < kHalves; ++half) {
+            const uint4* rows = reinterpret_cast<const uint4*>(v_buf + s * kBytes + half * kHalfBytes) + (lane & 7);
+#pragma unroll 8
+            for (int row = from + (lane >> 3); row < kTile; row += 4) {
+              const uint4 v = rows[row * 8];
+              carries |= ((v.x & kExp2) + kOne2) | ((v.y & kExp2) + kOne2) | ((v.z & kExp2) + kOne2) | ((v.w & kExp2) + kOne2);
             }
-            rows[i] = v;
-            odd = true;
+          }
+          const bool odd = __any_sync(0xffffffffu, (carries & 0x80008000u) != 0);
+          if (odd) {
+            constexpr uint32_t kExp = kExp2 & 0xffffu;
+            for (int half = 0; half < kHalves; ++half) {
+              uint32_t* words = reinterpret_cast<uint32_t*>(v_buf + s * kBytes + half * kHalfBytes) + lane;
+              for (int row = from; row < kTile; ++row) {
+                uint32_t e = words[row * 32];
+                if ((e & kExp) == kExp) e &= 0xffff0000u;
+                if (((e >> 16) & kExp) == kExp) e &= 0xffffu;
+                words[row * 32] = e;
+              }
+            }
           }
           if (odd) *reinterpret_cast<volatile int*>(&sh.odd_values) = 1;
           fence_async_smem();  // the replaced values -> the MMA's async-proxy reads
