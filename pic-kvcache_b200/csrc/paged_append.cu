@@ -224,8 +224,9 @@ __device__ __forceinline__ Target target(const Params& c, const Place& w) {
 // 16-byte pieces of 16/32-bit rows.  A thread takes two of them -- for neox the two
 // partners of a rotation, so that each is read once and one piece of the table serves
 // both -- in HPT heads, whose loads are in flight together and share the table's values.
-// HPT 4 at long prompts, 1 where there are too few tokens to fill the GPU (rule and
-// figures at pick_heads).
+// HPT 4 at long prompts, 1 where there are too few tokens to fill the GPU (more_heads).
+// A prompt of 16,384 tokens, 32 + 8 + 8 heads of 128: 77 us, 5.3 TB/s; 137 us when the loads
+// waited for slots and positions and each thread had one piece.
 template <typename T, typename TAB, int HPT>
 __global__ void __launch_bounds__(kThreads) append_kernel(const Params c) {
   constexpr int N = 16 / static_cast<int>(sizeof(T));
@@ -362,13 +363,76 @@ __device__ __forceinline__ void turn_piece(float (&x)[8], const float (&other)[8
   }
 }
 
-// 4-bit rows.  A lane takes the 8-value pieces at 8 p and D / 2 + 8 p of HPT heads of K or V
-// (and of the queries, which stay of their type): the two partners of a neox rotation over
-// the whole head, so nothing is read twice, and for D 128 one piece of each group of 64.  The
-// eight lanes of a D 128 row reduce both groups side by side, the four of a D 64 row their one.
-// EXTRA: neox over a part of the head, whose partners are read beside (they come from L1).
-// !WIDE: rows that are not aligned, or a rotary_dim that cuts a piece, value by value.
-template <typename T, typename TAB, int D, bool WIDE, bool EXTRA, int HPT>
+// Two elements of a 16-bit type in a word.
+template <typename T>
+struct Two;
+template <>
+struct Two<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float2 open(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  static __device__ __forceinline__ uint32_t least(uint32_t a, uint32_t b) {  // NaN if either is
+    const __nv_bfloat162 h = __hmin2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <>
+struct Two<__half> {
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float2 open(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+  static __device__ __forceinline__ uint32_t least(uint32_t a, uint32_t b) {
+    const __half2 h = __hmin2_nan(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+
+// Codes of 8 values in four words.  FAR: values may lie beyond
+// fp16's range.  Without them (x - low) / step is at least -1/2, since a 16-bit x in fp16's range
+// is off its fp16 form by 2^-25 at most and a step is 2^-24 at least, so that the nearest whole
+// number (the low bits of v + 1.5 * 2^23) can be cut to 0..15 as an integer, one instruction with
+// the subtraction of the float's upper bits.
+template <typename T, bool FAR>
+__device__ __forceinline__ uint32_t codes_of_words(const uint32_t (&w)[4], __half2 pair) {
+  const float step = __low2float(pair), base = __high2float(pair);
+  const float inverse = step > 0.0f ? __frcp_rn(step) : 0.0f;
+  uint32_t codes = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    // (packed products and sums would be contracted, so only the first difference is a pair's)
+    float2 v = __fadd2_rn(Two<T>::open(w[i]), make_float2(-base, -base));
+    v = make_float2(__fmul_rn(v.x, inverse), __fmul_rn(v.y, inverse));
+    if constexpr (FAR) v = make_float2(fminf(fmaxf(v.x, 0.0f), 15.0f), fminf(fmaxf(v.y, 0.0f), 15.0f));
+    v = make_float2(__fadd_rn(v.x, 12582912.0f), __fadd_rn(v.y, 12582912.0f));
+    const uint32_t x = __viaddmin_s32_relu(__float_as_int(v.x), -0x4b400000, 15);
+    const uint32_t y = __viaddmin_s32_relu(__float_as_int(v.y), -0x4b400000, 15);
+    codes += x * (1u << (8 * i)) + y * (16u << (8 * i));
+  }
+  return codes;
+}
+
+template <typename T>
+__device__ __noinline__ uint32_t far_codes(uint4 w, __half2 pair) {
+  const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+  return codes_of_words<T, true>(words, pair);
+}
+
+// 4-bit rows of 16-bit elements, aligned.  A lane takes the 8-value pieces at 8 p and
+// D / 2 + 8 p of HPT heads of K or V (and of the queries, which stay of their type): the two
+// partners of a neox rotation over the whole head, so nothing is read twice, and for D 128 one
+// piece of each group of 64.  The eight lanes of a D 128 row reduce both groups side by side,
+// the four of a D 64 row their one.  EXTRA: neox over a part of the head, whose partners are
+// read beside (they come from L1).
+// Bound by its instructions before HBM: 33 a value with one float at a time (60 us for a
+// prompt of 20,011 tokens and 8 heads, 1.7 TB/s), so minima and maxima, conversions and the
+// arithmetic go two values at a time.
+template <typename T, typename TAB, int D, bool EXTRA, int HPT>
 __global__ void __launch_bounds__(kThreads) append4_kernel(const Params c) {
   const Place w = place<HPT>(c, c.kv_heads, c.q_heads, D / 16);
   const bool is_q = w.plane == 2, neox = c.neox != 0;
@@ -383,41 +447,51 @@ __global__ void __launch_bounds__(kThreads) append4_kernel(const Params c) {
   for (int s = 0; s < 2; ++s) with[s] = at[s] >= c.rotary_dim ? at[s] : (at[s] < half ? at[s] + half : at[s] - half);
   // padding rows are read too: the loads wait for no slot or position
   Piece<T, 8> own[HPT][2], beside[EXTRA ? HPT : 1][2];
-  if constexpr (WIDE) {
 #pragma unroll
-    for (int i = 0; i < HPT; ++i)
-      if (w.head + i < heads) {
-        const T* row = reinterpret_cast<const T*>(src + (w.head + i) * src_hs);
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          own[i][s].load(row + at[s]);
-          if constexpr (EXTRA) beside[i][s].load(row + with[s]);
-        }
-      }
-  }
-  const Target g = target(c, w);
-  const bool turn = w.plane != 1 && c.rotary_dim > 0 && g.turned;
-  const TAB* table = static_cast<const TAB*>(c.table) + g.position * c.rotary_dim;
-  float cos[2][8], sin[2][8];
-  if constexpr (WIDE) {
-    if (turn) {
+  for (int i = 0; i < HPT; ++i)
+    if (w.head + i < heads) {
+      const T* row = reinterpret_cast<const T*>(src + (w.head + i) * src_hs);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        if (neox) {
-          const int i = at[s] < half ? at[s] : with[s];
-          if (at[s] < c.rotary_dim) {
-            load_n<TAB, 8, true>(table + i, cos[s]);
-            load_n<TAB, 8, true>(table + half + i, sin[s]);
-          }
-        } else if (at[s] < c.rotary_dim) {
-          float few[4];
-          load_n<TAB, 4, true>(table + at[s] / 2, few);
+        own[i][s].load(row + at[s]);
+        if constexpr (EXTRA) beside[i][s].load(row + with[s]);
+      }
+    } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) cos[s][j] = few[j];
-          load_n<TAB, 4, true>(table + half + at[s] / 2, few);
+      for (int s = 0; s < 2; ++s) {
+        own[i][s].v[0] = make_uint4(0, 0, 0, 0);
+        if constexpr (EXTRA) beside[i][s].v[0] = make_uint4(0, 0, 0, 0);
+      }
+    }
+  const Target g = target(c, w);
+  const bool turn = w.plane != 1 && c.rotary_dim > 0 && g.turned;
+  constexpr int kTables = EXTRA ? 2 : 1;
+  float cos[kTables][8], sin[kTables][8];  // neox over the whole head: one table piece for both partners;
+                                           // GPT-J: four pairs of each piece
+  if (turn) {
+    const TAB* table = static_cast<const TAB*>(c.table) + g.position * c.rotary_dim;
+    if constexpr (EXTRA) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) sin[s][j] = few[j];
-        }
+      for (int s = 0; s < 2; ++s) {
+        if (at[s] >= c.rotary_dim) continue;
+        const int i = min(at[s], with[s]);
+        load_n<TAB, 8, true>(table + i, cos[s]);
+        load_n<TAB, 8, true>(table + half + i, sin[s]);
+      }
+    } else if (neox) {
+      load_n<TAB, 8, true>(table + at[0], cos[0]);
+      load_n<TAB, 8, true>(table + half + at[0], sin[0]);
+    } else {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (at[s] >= c.rotary_dim) continue;
+        float few[4];
+        load_n<TAB, 4, true>(table + at[s] / 2, few);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) cos[0][4 * s + j] = few[j];
+        load_n<TAB, 4, true>(table + half + at[s] / 2, few);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sin[0][4 * s + j] = few[j];
       }
     }
   }
@@ -425,73 +499,84 @@ __global__ void __launch_bounds__(kThreads) append4_kernel(const Params c) {
   const int64_t scale_at = g.block * c.scale_block_stride + g.row * c.scale_slot_stride;
 #pragma unroll
   for (int i = 0; i < HPT; ++i) {
-    const bool here = w.head + i < heads && (is_q || g.stored);
-    float x[2][8];
-    if (here && g.turned) {
-      if constexpr (WIDE) {
-        float other[2][8];
+    uint32_t word[2][4];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) word[s][j] = reinterpret_cast<const uint32_t*>(own[i][s].v)[j];
+    if (turn) {
+      if constexpr (EXTRA) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          float x[8], other[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = own[i][s][j], other[j] = beside[i][s][j];
+          turn_piece(x, other, at[s], c.rotary_dim, true, cos[s], sin[s]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) word[s][j] = Two<T>::pack(x[2 * j], x[2 * j + 1]);
+        }
+      } else if (neox) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {  // (the packed product and sum would be contracted)
+          const float2 a = Two<T>::open(word[0][j]), b = Two<T>::open(word[1][j]);
+          const float c0 = cos[0][2 * j], c1 = cos[0][2 * j + 1], s0 = sin[0][2 * j], s1 = sin[0][2 * j + 1];
+          word[0][j] = Two<T>::pack(turn_first(a.x, b.x, c0, s0), turn_first(a.y, b.y, c1, s1));
+          word[1][j] = Two<T>::pack(turn_second(a.x, b.x, c0, s0), turn_second(a.y, b.y, c1, s1));
+        }
+      } else {
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            x[s][j] = own[i][s][j];
-            other[s][j] = EXTRA ? beside[EXTRA ? i : 0][s][j] : own[i][1 - s][j];
+          for (int j = 0; j < 4; ++j) {
+            if (at[s] >= c.rotary_dim) continue;
+            const float2 x = Two<T>::open(word[s][j]);
+            const float co = cos[0][4 * s + j], si = sin[0][4 * s + j];
+            word[s][j] = Two<T>::pack(turn_first(x.x, x.y, co, si), turn_second(x.x, x.y, co, si));
           }
-        if (turn) {
-#pragma unroll
-          for (int s = 0; s < 2; ++s) turn_piece(x[s], other[s], at[s], c.rotary_dim, neox, cos[s], sin[s]);
-        }
-      } else {
-        const T* row = reinterpret_cast<const T*>(src + (w.head + i) * src_hs);
-#pragma unroll
-        for (int s = 0; s < 2; ++s) rotated<T, TAB, 8, false>(row, at[s], table, turn ? c.rotary_dim : 0, neox, x[s]);
       }
-    } else {
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[s][j] = 0.0f;
     }
-    if (here && is_q) {
+    if (is_q && w.head + i < heads) {
       T* out = reinterpret_cast<T*>(c.query_out + w.token * c.qo_ts + (w.head + i) * c.qo_hs);
 #pragma unroll
-      for (int s = 0; s < 2; ++s) store_n<T, 8, WIDE>(out + at[s], x[s]);
+      for (int s = 0; s < 2; ++s)  // zeros at a position outside the table
+        *reinterpret_cast<uint4*>(out + at[s]) =
+            g.turned ? make_uint4(word[s][0], word[s][1], word[s][2], word[s][3]) : make_uint4(0, 0, 0, 0);
     }
-    float low[2], high[2], odd[2];
+    // (lowest, -highest) of each piece in one word; NaN where a value is
+    uint32_t ends[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      low[s] = INFINITY, high[s] = -INFINITY, odd[s] = 0.0f;
+      uint32_t low = word[s][0], high = word[s][0] ^ 0x80008000u;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        // the row as the element type holds it: 4-bit pages hold what 16-bit pages would
-        x[s][j] = rnd<T>(x[s][j]);
-        low[s] = fminf(low[s], x[s][j]);
-        high[s] = fmaxf(high[s], x[s][j]);
-        odd[s] = fmaf(x[s][j], 0.0f, odd[s]);  // NaN once a value is NaN or infinite
+      for (int j = 1; j < 4; ++j) {
+        low = Two<T>::least(low, word[s][j]);
+        high = Two<T>::least(high, word[s][j] ^ 0x80008000u);
       }
+      // the words' two halves against each other
+      ends[s] = Two<T>::least(__byte_perm(low, high, 0x5410), __byte_perm(low, high, 0x7632));
     }
-    if constexpr (D == 64) {
-      low[0] = fminf(low[0], low[1]), high[0] = fmaxf(high[0], high[1]), odd[0] += odd[1];
-    }
+    if constexpr (D == 64) ends[0] = Two<T>::least(ends[0], ends[1]);
     // every lane of the warp is here: the lanes of a row reduce with their neighbours
     constexpr int kGroups = D / kGroup;
     __half2 pair[2];
+    bool far[2];
 #pragma unroll
     for (int s = 0; s < kGroups; ++s) {
 #pragma unroll
-      for (int o = D / 32; o >= 1; o >>= 1) {
-        low[s] = fminf(low[s], __shfl_xor_sync(0xffffffffu, low[s], o));
-        high[s] = fmaxf(high[s], __shfl_xor_sync(0xffffffffu, high[s], o));
-      }
-      const uint32_t votes = __ballot_sync(0xffffffffu, odd[s] != 0.0f);  // unequal also when NaN
-      constexpr uint32_t kLanes = D / 16;
-      pair[s] = step_of(low[s], high[s], (votes >> (threadIdx.x & (32u - kLanes))) & ((1u << kLanes) - 1u));
+      for (int o = D / 32; o >= 1; o >>= 1) ends[s] = Two<T>::least(ends[s], __shfl_xor_sync(0xffffffffu, ends[s], o));
+      const float2 e = Two<T>::open(ends[s]);
+      far[s] = !(fmaxf(-e.x, -e.y) <= kHalfMax);
+      pair[s] = step_of(e.x, -e.y, !(fabsf(e.x) + fabsf(e.y) < INFINITY));
     }
-    if constexpr (D == 64) pair[1] = pair[0];
-    if (!here || is_q) continue;
+    if constexpr (D == 64) pair[1] = pair[0], far[1] = far[0];
+    if (is_q || !g.stored || w.head + i >= heads) continue;
     char* dst = (w.plane == 0 ? c.k_cache : c.v_cache) + row_at + (w.head + i) * c.head_stride;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) *reinterpret_cast<uint32_t*>(dst + at[s] / 2) = codes_of(x[s], pair[s]);
+    for (int s = 0; s < 2; ++s) {
+      const uint32_t codes = far[s] ? far_codes<T>(make_uint4(word[s][0], word[s][1], word[s][2], word[s][3]), pair[s])
+                                    : codes_of_words<T, false>(word[s], pair[s]);
+      *reinterpret_cast<uint32_t*>(dst + at[s] / 2) = codes;
+    }
     if (w.piece == 0) {
       char* sc = (w.plane == 0 ? c.k_scales : c.v_scales) + scale_at + (w.head + i) * c.scale_head_stride;
       if constexpr (D == 64) {
@@ -501,6 +586,70 @@ __global__ void __launch_bounds__(kThreads) append4_kernel(const Params c) {
             make_uint2(*reinterpret_cast<const uint32_t*>(&pair[0]), *reinterpret_cast<const uint32_t*>(&pair[1]));
       }
     }
+  }
+}
+
+// The same for fp32 elements, for rows that are not aligned and for a rotary_dim that cuts a
+// piece of 8: value by value, one head per thread.
+template <typename T, typename TAB, int D>
+__global__ void __launch_bounds__(kThreads) append4_narrow_kernel(const Params c) {
+  const Place w = place<1>(c, c.kv_heads, c.q_heads, D / 16);
+  const bool is_q = w.plane == 2;
+  const char* src = is_q ? c.query + w.token * c.query_ts + w.head * c.query_hs
+                         : (w.plane == 0 ? c.key + w.token * c.key_ts + w.head * c.key_hs
+                                         : c.value + w.token * c.value_ts + w.head * c.value_hs);
+  const Target g = target(c, w);
+  const int at[2] = {8 * w.piece, D / 2 + 8 * w.piece};
+  const bool here = w.real && g.turned && (is_q || g.stored);
+  float x[2][8], low[2], high[2], odd[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    if (here) {
+      rotated<T, TAB, 8, false>(reinterpret_cast<const T*>(src), at[s],
+                                static_cast<const TAB*>(c.table) + g.position * c.rotary_dim,
+                                w.plane == 1 ? 0 : c.rotary_dim, c.neox != 0, x[s]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[s][j] = 0.0f;
+    }
+    low[s] = INFINITY, high[s] = -INFINITY, odd[s] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[s][j] = rnd<T>(x[s][j]);  // the row as the element type holds it
+      low[s] = fminf(low[s], x[s][j]);
+      high[s] = fmaxf(high[s], x[s][j]);
+      odd[s] = fmaf(x[s][j], 0.0f, odd[s]);  // NaN once a value is NaN or infinite
+    }
+  }
+  if (is_q && w.real) {
+    T* out = reinterpret_cast<T*>(c.query_out + w.token * c.qo_ts + w.head * c.qo_hs);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) store_n<T, 8, false>(out + at[s], x[s]);
+  }
+  if constexpr (D == 64) low[0] = fminf(low[0], low[1]), high[0] = fmaxf(high[0], high[1]), odd[0] += odd[1];
+  constexpr int kGroups = D / kGroup;
+  __half2 pair[2];
+#pragma unroll
+  for (int s = 0; s < kGroups; ++s) {
+#pragma unroll
+    for (int o = D / 32; o >= 1; o >>= 1) {
+      low[s] = fminf(low[s], __shfl_xor_sync(0xffffffffu, low[s], o));
+      high[s] = fmaxf(high[s], __shfl_xor_sync(0xffffffffu, high[s], o));
+    }
+    const uint32_t votes = __ballot_sync(0xffffffffu, odd[s] != 0.0f);  // unequal also when NaN
+    constexpr uint32_t kLanes = D / 16;
+    pair[s] = step_of(low[s], high[s], (votes >> (threadIdx.x & (32u - kLanes))) & ((1u << kLanes) - 1u));
+  }
+  if constexpr (D == 64) pair[1] = pair[0];
+  if (!here || is_q) return;
+  char* dst = (w.plane == 0 ? c.k_cache : c.v_cache) + g.block * c.block_stride + g.row * c.slot_stride + w.head * c.head_stride;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) *reinterpret_cast<uint32_t*>(dst + at[s] / 2) = codes_of(x[s], pair[s]);
+  if (w.piece == 0) {
+    __half2* sc = reinterpret_cast<__half2*>((w.plane == 0 ? c.k_scales : c.v_scales) + g.block * c.scale_block_stride +
+                                             g.row * c.scale_slot_stride + w.head * c.scale_head_stride);
+#pragma unroll
+    for (int s = 0; s < kGroups; ++s) sc[s] = pair[s];
   }
 }
 
@@ -575,9 +724,10 @@ inline int64_t units_of(int64_t kv_heads, int64_t q_heads, int64_t pieces, int64
   return (2 * ((kv_heads + hpt - 1) / hpt) + (q_heads + hpt - 1) / hpt) * pieces;
 }
 
-// Whether a thread takes four heads: once one head per thread would fill the GPU's resident
-// threads anyway.
-inline bool four_heads(int64_t units, int64_t tokens) { return units * tokens >= int64_t(kSmCount) * 2048; }
+// Whether a thread takes several heads: once one head per thread would fill the GPU's resident
+// threads anyway.  Four of them for 16/32-bit pages and the read-back; two for 4-bit pages, which
+// want the registers (20,011 tokens: 74 us with four).
+inline bool more_heads(int64_t units, int64_t tokens) { return units * tokens >= int64_t(kSmCount) * 2048; }
 
 int check_units(int64_t units) {
   CB_REQUIRE(units < (int64_t(1) << 23), "row too wide (%lld pieces)", (long long)units);
@@ -585,16 +735,20 @@ int check_units(int64_t units) {
 }
 
 template <typename T, typename TAB, int D>
-void launch4(const Params& c, dim3 grid, bool wide, bool four, cudaStream_t s) {
-  const bool extra = c.neox && c.rotary_dim > 0 && c.rotary_dim < D;
-  if (!wide)
-    append4_kernel<T, TAB, D, false, false, 1><<<grid, kThreads, 0, s>>>(c);
-  else if (extra)
-    four ? append4_kernel<T, TAB, D, true, true, 4><<<grid, kThreads, 0, s>>>(c)
-         : append4_kernel<T, TAB, D, true, true, 1><<<grid, kThreads, 0, s>>>(c);
-  else
-    four ? append4_kernel<T, TAB, D, true, false, 4><<<grid, kThreads, 0, s>>>(c)
-         : append4_kernel<T, TAB, D, true, false, 1><<<grid, kThreads, 0, s>>>(c);
+void launch4(const Params& c, dim3 grid, bool wide, bool more, cudaStream_t s) {
+  if constexpr (sizeof(T) == 2) {
+    const bool extra = c.neox && c.rotary_dim > 0 && c.rotary_dim < D;
+    if (wide) {
+      if (extra)
+        more ? append4_kernel<T, TAB, D, true, 2><<<grid, kThreads, 0, s>>>(c)
+             : append4_kernel<T, TAB, D, true, 1><<<grid, kThreads, 0, s>>>(c);
+      else
+        more ? append4_kernel<T, TAB, D, false, 2><<<grid, kThreads, 0, s>>>(c)
+             : append4_kernel<T, TAB, D, false, 1><<<grid, kThreads, 0, s>>>(c);
+      return;
+    }
+  }
+  append4_narrow_kernel<T, TAB, D><<<grid, kThreads, 0, s>>>(c);
 }
 
 template <bool FOUR, typename T, typename TAB>
@@ -604,17 +758,17 @@ int launch(Params& c, bool wide, cudaStream_t s) {
   const int64_t units = units_of(c.kv_heads, c.q_heads, pieces, 1);
   const int rc = check_units(units);
   if (rc != CB_OK) return rc;
-  const bool four = wide && four_heads(units, c.tokens);
-  const dim3 grid = lay_out(c, four ? units_of(c.kv_heads, c.q_heads, pieces, 4) : units, c.tokens);
+  const bool more = wide && more_heads(units, c.tokens);
+  const dim3 grid = lay_out(c, more ? units_of(c.kv_heads, c.q_heads, pieces, FOUR ? 2 : 4) : units, c.tokens);
   if constexpr (FOUR) {
     if (c.head_size == 64)
-      launch4<T, TAB, 64>(c, grid, wide, four, s);
+      launch4<T, TAB, 64>(c, grid, wide, more, s);
     else
-      launch4<T, TAB, 128>(c, grid, wide, four, s);
+      launch4<T, TAB, 128>(c, grid, wide, more, s);
   } else {
     if (!wide)
       append_narrow_kernel<T, TAB><<<grid, kThreads, 0, s>>>(c);
-    else if (four)
+    else if (more)
       append_kernel<T, TAB, 4><<<grid, kThreads, 0, s>>>(c);
     else
       append_kernel<T, TAB, 1><<<grid, kThreads, 0, s>>>(c);
@@ -638,7 +792,7 @@ int dispatch(Params& c, int dtype, int table_dtype, bool wide, cudaStream_t s) {
 template <typename T>
 void launch_gather4(GatherParams& c, bool wide, cudaStream_t s) {
   const int64_t pieces = c.head_size / 16, units = units_of(c.heads, 0, pieces, 1);
-  const bool four = wide && four_heads(units, c.tokens);
+  const bool four = wide && more_heads(units, c.tokens);
   const dim3 grid = lay_out(c, four ? units_of(c.heads, 0, pieces, 4) : units, c.tokens);
   if (!wide)
     gather4_kernel<T, false, 1><<<grid, kThreads, 0, s>>>(c);
@@ -776,7 +930,8 @@ extern "C" int cb_append_paged_kv4(const void* key, int64_t key_token_stride, in
   rc = append::check_pages4(block_stride, slot_stride, head_stride, scale_block_stride, scale_slot_stride,
                             scale_head_stride, k_codes, v_codes, k_scales, v_scales, head_size);
   if (rc != CB_OK) return rc;
-  return append::dispatch<true>(c, dtype, cos_sin_dtype, append::wide_rows(c, 8, 16, 0), reinterpret_cast<cudaStream_t>(stream));
+  return append::dispatch<true>(c, dtype, cos_sin_dtype, dtype != CB_DTYPE_FP32 && append::wide_rows(c, 8, 16, 0),
+                                reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" int cb_gather_paged_kv4(const void* k_codes, const void* v_codes, int64_t block_stride, int64_t slot_stride,
