@@ -29,7 +29,10 @@
 //     transposing ldmatrix of 16-bit units (four codes of a key) pairs the same
 //     codes of two keys.  P step'_G is rounded to fp16 (11 bits: 2^-12 relative,
 //     against the 2^-9 of a bf16 output) once per group and transposed by
-//     movmatrix.  M also carries the exponent of the largest step' so that a
+//     movmatrix.  The roundings weigh with codes less 8, not with codes: 8 times the
+//     sum of the rounded factors (one more product, of ones) is taken off again and
+//     the low terms are taken at code 8, so that a row's offset does not multiply them
+//     (fp16 outputs of rows around 0: 3.4e-4 off without, 2.1e-4 for one rounding).  M also carries the exponent of the largest step' so that a
 //     factor stays in fp16's range whatever the values' size: at most 2^15, 2^10
 //     when M is set.  M moves only when a factor would pass that, which each lane
 //     sees for itself: the common tile needs no maximum over the warp.
@@ -180,7 +183,7 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;
+constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u, kEight = 0x00080008u;
 
 template <int D>
 struct Tile {
@@ -444,7 +447,8 @@ __global__ void __launch_bounds__(kThreads, 2) attention4_kernel(const __grid_co
       last[j] = len - piece.tokens + min(row0 + col, piece.tokens * c.groups - 1) / c.groups;
     }
 
-    float o[kChunks][2][4], low[kGroups][2], m[2], l[2];
+    float o[kChunks][2][4], eights[4], low[kGroups][2], m[2], l[2];
+    eights[0] = eights[1] = eights[2] = eights[3] = 0.0f;
     m[0] = m[1] = -INFINITY;
     l[0] = l[1] = 0.0f;
 #pragma unroll
@@ -540,6 +544,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention4_kernel(const __grid_co
             l[j] *= keep;
 #pragma unroll
             for (int G = 0; G < kGroups; ++G) low[G][j] *= keep;
+            eights[j] *= keep, eights[j + 2] *= keep;
 #pragma unroll
             for (int ch = 0; ch < kChunks; ++ch)
 #pragma unroll
@@ -566,13 +571,14 @@ __global__ void __launch_bounds__(kThreads, 2) attention4_kernel(const __grid_co
 #pragma unroll
           for (int G = 0; G < kGroups; ++G) {
             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&vpair[mt][r][G]));
+            const float middle = fmaf(8.0f, f.x, f.y);  // of a row's values: what code 8 stands for
             float by[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               // an unseen row gives nothing whatever it holds
               const bool none = CUT && w[mt][r * 2 + j] == -INFINITY;
               by[j] = none ? 0.0f : p[j] * f.x;
-              low[G][j] = none ? low[G][j] : fmaf(p[j], f.y, low[G][j]);
+              low[G][j] = none ? low[G][j] : fmaf(p[j], middle, low[G][j]);
             }
             b[G][r] = transposed(pack(by[0], by[1]));
           }
@@ -586,6 +592,8 @@ __global__ void __launch_bounds__(kThreads, 2) attention4_kernel(const __grid_co
             const uint32_t near = x[j & 2] >> (8 * (j & 1)), far = x[(j & 2) + 1] >> (8 * (j & 1));
             mma(o[G * 2 + (j >> 1)][j & 1], near & kEven, near & kOdd, far & kEven, far & kOdd, b[G][0], b[G][1]);
           }
+          // 8 times the sums of the rounded factors, the first group's in rows 0-7
+          mma(eights, G == 0 ? kEight : 0u, G == 0 ? 0u : kEight, G == 0 ? kEight : 0u, G == 0 ? 0u : kEight, b[G][0], b[G][1]);
         }
       }
     };
@@ -621,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention4_kernel(const __grid_co
         row_m[warp][row] = m[j];
         row_l[warp][row] = l[j];
 #pragma unroll
-        for (int G = 0; G < kGroups; ++G) low_sum[warp][row][G] = low[G][j];
+        for (int G = 0; G < kGroups; ++G) low_sum[warp][row][G] = low[G][j] - eights[2 * G + j] * 16777216.0f;
       }
     }
     __syncthreads();  // every warp is done with its ring as well
