@@ -42,17 +42,20 @@ class PagedKV4:
 
     def __post_init__(self) -> None:
         codes, scales = self.codes, self.scales
-        if codes.ndim != 5 or codes.shape[0] != 2 or codes.dtype != torch.uint8:
+        shape = codes.shape
+        if len(shape) != 5 or shape[0] != 2 or codes.dtype != torch.uint8:
             raise ValueError("codes must be uint8 [2, blocks, heads, block_size, head_size // 2]")
-        if codes.shape[4] not in (32, 64):
-            raise NotImplementedError(f"4-bit pages hold heads of 64 or 128 values, not {2 * codes.shape[4]}")
-        if scales.dtype != torch.float16 or tuple(scales.shape) != (*codes.shape[:4], codes.shape[4] * 2 // GROUP, 2):
+        _, blocks, heads, rows, half = shape
+        if half not in (32, 64):
+            raise NotImplementedError(f"4-bit pages hold heads of 64 or 128 values, not {2 * half}")
+        if scales.dtype != torch.float16 or scales.shape != (2, blocks, heads, rows, half // 32, 2):
             raise ValueError("scales must be float16 [2, blocks, heads, block_size, head_size // 64, 2]")
         if codes.device != scales.device:
             raise ValueError("codes and scales must live on one device")
-        if codes.shape[2] == 0 or codes.shape[3] == 0:
+        if heads == 0 or rows == 0:
             raise ValueError("4-bit pages need at least one head and one row")
-        if codes.stride(4) != 1 or scales.stride(5) != 1 or (scales.shape[4] > 1 and scales.stride(4) != 2):
+        *_, group, pair = scales.stride()
+        if codes.stride(4) != 1 or pair != 1 or (half == 64 and group != 2):
             raise ValueError("the rows of 4-bit pages must be contiguous")
 
     @classmethod
@@ -112,29 +115,56 @@ def current_handle() -> int:
 
 def _index(name: str, index: torch.Tensor, count: int, device: torch.device, low: int | None, high: int) -> torch.Tensor:
     """One int64 per token on ``device``; host values are range-checked first."""
-    if index.ndim != 1 or index.numel() != count:
+    if index.ndim != 1 or index.shape[0] != count:
         raise ValueError(f"{name} must hold one entry per token ({count}), got shape {tuple(index.shape)}")
+    if index.dtype == torch.long and index.device == device:
+        return index if index.is_contiguous() else index.contiguous()
     if index.is_floating_point() or index.dtype == torch.bool:
         raise ValueError(f"{name} must be whole numbers, not {index.dtype}")
-    if index.device.type == "cpu" and count:
-        if (low is not None and int(index.min()) < low) or int(index.max()) >= high:
+    if index.device.type == "cpu":
+        if count and ((low is not None and int(index.min()) < low) or int(index.max()) >= high):
             raise IndexError(f"{name} out of range: [{int(index.min())}, {int(index.max())}] for {high}")
-    elif index.device.type != "cpu" and index.device != device:
+    elif index.device != device:
         raise ValueError(f"{name} must live on the host or on {device}")
-    if index.dtype != torch.long or index.device != device:
-        index = index.to(device=device, dtype=torch.long)
-    return index.contiguous()
+    return index.to(device=device, dtype=torch.long).contiguous()
 
 
-def _rows(name: str, tensor: torch.Tensor, like: torch.Tensor) -> None:
-    if tensor.ndim != 3:
-        raise ValueError(f"{name} must be [tokens, heads, head_size], got {tuple(tensor.shape)}")
-    if tensor.shape[0] != like.shape[0] or tensor.shape[2] != like.shape[2]:
-        raise ValueError(f"{name} {tuple(tensor.shape)} does not match the keys {tuple(like.shape)}")
-    if tensor.dtype != like.dtype or tensor.device != like.device:
-        raise ValueError(f"{name} must share the keys' dtype and device")
-    if tensor.shape[2] > 1 and tensor.stride(2) != 1:
-        raise ValueError(f"the values of a head of {name} must be contiguous")
+def _check_rows(key: torch.Tensor, value: torch.Tensor, query: torch.Tensor | None) -> tuple[int, int, int]:
+    """(tokens, kv_heads, head_size) of rows that go together."""
+    shape, dtype, device = key.shape, key.dtype, key.device
+    if len(shape) != 3:
+        raise ValueError(f"key must be [tokens, heads, head_size], got {tuple(shape)}")
+    if value.shape != shape:
+        raise ValueError(f"key and value must have the same shape, not {tuple(shape)} and {tuple(value.shape)}")
+    if value.dtype != dtype or value.device != device:
+        raise ValueError("value must share the keys' dtype and device")
+    if query is not None:
+        q = query.shape
+        if len(q) != 3 or q[0] != shape[0] or q[2] != shape[2]:
+            raise ValueError(f"query {tuple(q)} does not match the keys {tuple(shape)}")
+        if query.dtype != dtype or query.device != device:
+            raise ValueError("query must share the keys' dtype and device")
+    if shape[2] > 1 and (key.stride(2) != 1 or value.stride(2) != 1 or (query is not None and query.stride(2) != 1)):
+        raise ValueError("the values of a head must be contiguous in key, value and query")
+    _native.dtype_code(dtype)
+    return shape
+
+
+def _page_planes(kv_layer: KVLayer, block_size: int) -> tuple:
+    """(K address, V address, shape, strides, dtype, device) of 16/32-bit pages [blocks, rows, heads, head_size].
+
+    The merged layouts are taken apart by arithmetic: describe_paged's views are most of a
+    decode step's call.  Whatever is unusual goes through it."""
+    if isinstance(kv_layer, torch.Tensor) and kv_layer.ndim == 5:
+        shape, strides = kv_layer.shape, kv_layer.stride()
+        plane = 0 if shape[0] == 2 else 1 if shape[1] == 2 else None
+        if plane is not None and 0 < block_size <= shape[2]:
+            key = kv_layer.data_ptr()
+            return (key, key + strides[plane] * kv_layer.element_size(), (shape[1 - plane], *shape[2:]),
+                    (strides[1 - plane], *strides[2:]), kv_layer.dtype, kv_layer.device)
+    paged = describe_paged(kv_layer, block_size)
+    return (paged.key.data_ptr(), paged.value.data_ptr(), tuple(paged.key.shape), paged.key.stride(), paged.dtype,
+            paged.device)
 
 
 def _rotation(rotary_emb, head_size: int, key: torch.Tensor) -> tuple:
@@ -155,30 +185,35 @@ def _rotation(rotary_emb, head_size: int, key: torch.Tensor) -> tuple:
         int(bool(rotary_emb.is_neox_style))
 
 
-def _append(entry: str, rotary_emb, positions, key, value, query, slot_mapping, num_slots: int, block_size: int,
-            num_blocks: int, pages: tuple, stream) -> torch.Tensor | None:
+def _append(entry: str, rotary_emb, positions, key, value, query, slot_mapping, num_blocks: int, block_size: int,
+            pages: tuple, stream) -> torch.Tensor | None:
     tokens, heads, head_size = key.shape
+    device = key.device
     table, table_code, max_position, rotary_dim, neox = _rotation(rotary_emb, head_size, key)
-    with on_device(key.device, stream):
-        slots = _index("slot_mapping", slot_mapping, tokens, key.device, None, num_slots)
-        where = None
+    with on_device(device, stream):
+        slots = _index("slot_mapping", slot_mapping, tokens, device, None, num_blocks * block_size)
+        where = 0
         if rotary_dim:
             if positions is None:
                 raise ValueError("a rotation needs one position per token")
-            where = _index("positions", positions, tokens, key.device, 0, max_position)
-        turned = None if query is None else torch.empty(query.shape, dtype=query.dtype, device=query.device)
+            positions = _index("positions", positions, tokens, device, 0, max_position)
+            where = positions.data_ptr()
+        turned, q_heads, q = None, 0, (0, 0, 0, 0, 0, 0)
+        size = key.element_size()
+        if query is not None:
+            turned = torch.empty_like(query, memory_format=torch.contiguous_format)
+            q_heads = query.shape[1]
+            from_token, from_head, _ = query.stride()
+            q = (query.data_ptr(), from_token * size, from_head * size, turned.data_ptr(), q_heads * head_size * size,
+                 head_size * size)
         if tokens == 0:
             return turned
-        size = key.element_size()
-        strides = [s * size for t in (key, value) for s in t.stride()[:2]]
-        q = (0, 0, 0, 0, 0, 0) if query is None else (
-            query.data_ptr(), query.stride(0) * size, query.stride(1) * size,
-            turned.data_ptr(), turned.stride(0) * size, turned.stride(1) * size)
-        _native.call(entry, key.data_ptr(), strides[0], strides[1], value.data_ptr(), strides[2], strides[3], *q, tokens,
-                     0 if query is None else query.shape[1], heads, head_size, _native.dtype_code(key.dtype),
-                     0 if where is None else where.data_ptr(), 0 if table is None else table.data_ptr(), table_code,
-                     max_position, rotary_dim, neox, *pages, num_blocks, block_size, slots.data_ptr(),
-                     current_handle())
+        key_token, key_head, _ = key.stride()
+        value_token, value_head, _ = value.stride()
+        _native.call(entry, key.data_ptr(), key_token * size, key_head * size, value.data_ptr(), value_token * size,
+                     value_head * size, *q, tokens, q_heads, heads, head_size, _native.DTYPE_CODES[key.dtype], where,
+                     0 if table is None else table.data_ptr(), table_code, max_position, rotary_dim, neox, *pages,
+                     num_blocks, block_size, slots.data_ptr(), current_handle())
         return turned
 
 
@@ -210,25 +245,20 @@ def append_paged_kv(
     outside the cache, or a position outside the table, leaves the pages as they were (and
     gives a zero query row).
     """
-    _rows("key", key, key)
-    _rows("value", value, key)
-    if value.shape != key.shape:
-        raise ValueError("key and value must have the same shape")
-    if query is not None:
-        _rows("query", query, key)
-    paged = describe_paged(kv_layer, block_size)
-    _native.require_cuda(paged.key, key)
-    _native.dtype_code(key.dtype)
-    if key.dtype != paged.dtype or key.device != paged.device:
+    _, heads, head_size = _check_rows(key, value, query)
+    k_pages, v_pages, shape, strides, dtype, device = _page_planes(kv_layer, block_size)
+    if not key.is_cuda or device.type != "cuda":
+        _native.require_cuda(key, *(kv_layer if not isinstance(kv_layer, torch.Tensor) else (kv_layer,)))
+    if key.dtype != dtype or key.device != device:
         raise ValueError("keys must match the KV cache dtype and device")
-    if paged.key.ndim != 4 or tuple(paged.key.shape[2:]) != tuple(key.shape[1:]):
-        raise ValueError(f"pages {tuple(paged.key.shape)} do not hold rows of {tuple(key.shape[1:])}")
-    if paged.key.shape[3] > 1 and paged.key.stride(3) != 1:
+    if len(shape) != 4 or shape[2] != heads or shape[3] != head_size:
+        raise ValueError(f"pages {tuple(shape)} do not hold rows of {(heads, head_size)}")
+    if head_size > 1 and strides[3] != 1:
         raise ValueError("the values of a head must be contiguous in the pages")
-    pages = (paged.key.data_ptr(), paged.value.data_ptr(), paged.block_stride, paged.slot_stride,
-             paged.key.stride(2) * key.element_size())
-    return _append("cb_append_paged_kv", rotary_emb, positions, key, value, query, slot_mapping,
-                   paged.num_blocks * paged.block_size, paged.block_size, paged.num_blocks, pages, stream)
+    size = key.element_size()
+    pages = (k_pages, v_pages, strides[0] * size, strides[1] * size, strides[2] * size)
+    return _append("cb_append_paged_kv", rotary_emb, positions, key, value, query, slot_mapping, shape[0], block_size,
+                   pages, stream)
 
 
 def append_paged_kv4(
@@ -248,20 +278,16 @@ def append_paged_kv4(
     nearest.  Values beyond +-65504 are held at that; a group with a NaN or an infinity reads
     as NaN.
     """
-    _rows("key", key, key)
-    _rows("value", value, key)
-    if value.shape != key.shape:
-        raise ValueError("key and value must have the same shape")
-    if query is not None:
-        _rows("query", query, key)
-    _native.require_cuda(cache.codes, key)
-    _native.dtype_code(key.dtype)
+    _, heads, head_size = _check_rows(key, value, query)
+    if not key.is_cuda or not cache.codes.is_cuda:
+        _native.require_cuda(cache.codes, key)
     if key.device != cache.device:
         raise ValueError("keys must live on the cache's device")
-    if tuple(key.shape[1:]) != (cache.num_heads, cache.head_size):
-        raise ValueError(f"the cache holds rows of {(cache.num_heads, cache.head_size)}, not {tuple(key.shape[1:])}")
-    return _append("cb_append_paged_kv4", rotary_emb, positions, key, value, query, slot_mapping,
-                   cache.num_blocks * cache.block_size, cache.block_size, cache.num_blocks, cache._pages(), stream)
+    _, num_blocks, cache_heads, rows, half = cache.codes.shape
+    if heads != cache_heads or head_size != 2 * half:
+        raise ValueError(f"the cache holds rows of {(cache_heads, 2 * half)}, not {(heads, head_size)}")
+    return _append("cb_append_paged_kv4", rotary_emb, positions, key, value, query, slot_mapping, num_blocks, rows,
+                   cache._pages(), stream)
 
 
 def gather_paged_kv4(
@@ -276,26 +302,26 @@ def gather_paged_kv4(
     A negative slot (padding) reads as zeros; so does, on the device, one outside the cache
     (IndexError for host slots).
     """
-    _native.require_cuda(cache.codes)
-    tokens = int(slot_mapping.numel())
-    shape = (2, tokens, cache.num_heads, cache.head_size)
+    if not cache.codes.is_cuda:
+        _native.require_cuda(cache.codes)
+    _, num_blocks, heads, rows, half = cache.codes.shape
+    tokens, device = slot_mapping.numel(), cache.device
+    shape = (2, tokens, heads, 2 * half)
     code = _native.dtype_code(dtype)
     if out is not None:
         if tuple(out.shape) != shape:
             raise ValueError(f"gather output has shape {tuple(out.shape)}, expected {shape}")
-        if out.dtype != dtype or out.device != cache.device:
+        if out.dtype != dtype or out.device != device:
             raise ValueError("gather output must match the dtype and the cache's device")
         if out.stride(3) != 1:
             raise ValueError("the values of a head must be contiguous in the output")
-    with on_device(cache.device, stream):
-        slots = _index("slot_mapping", slot_mapping, tokens, cache.device, None, cache.num_blocks * cache.block_size)
-        result = out if out is not None else torch.empty(shape, dtype=dtype, device=cache.device)
+    with on_device(device, stream):
+        slots = _index("slot_mapping", slot_mapping, tokens, device, None, num_blocks * rows)
+        result = out if out is not None else torch.empty(shape, dtype=dtype, device=device)
         if tokens == 0:
             return result
         size = result.element_size()
-        codes_k, codes_v, block_stride, slot_stride, head_stride, *scales = cache._pages()
-        _native.call("cb_gather_paged_kv4", codes_k, codes_v, block_stride, slot_stride, head_stride, *scales,
-                     cache.num_blocks, cache.block_size, cache.num_heads, cache.head_size, slots.data_ptr(), tokens,
-                     result.data_ptr(), result.stride(0) * size, result.stride(1) * size, result.stride(2) * size, code,
-                     current_handle())
+        plane, token, head, _ = result.stride()
+        _native.call("cb_gather_paged_kv4", *cache._pages(), num_blocks, rows, heads, 2 * half, slots.data_ptr(), tokens,
+                     result.data_ptr(), plane * size, token * size, head * size, code, current_handle())
         return result

@@ -103,7 +103,7 @@ def blend_attention(
 def _int32(name: str, tensor: torch.Tensor, device: torch.device, ndim: int) -> None:
     if tensor.dtype != torch.int32 or tensor.device != device or tensor.ndim != ndim:
         raise ValueError(f"{name} must be a {ndim}-dimensional int32 tensor on {device}")
-    if tensor.shape[-1] > 1 and tensor.stride(-1) != 1:
+    if tensor.stride(-1) != 1 and tensor.shape[-1] > 1:
         raise ValueError(f"{name} must be contiguous")
 
 
@@ -152,45 +152,49 @@ def paged_attention4(
     """
     if query.ndim != 3:
         raise ValueError("query must be [tokens, q_heads, head_size]")
-    if query.dtype not in (torch.bfloat16, torch.float16):
-        raise NotImplementedError(f"queries must be bfloat16 or float16, not {query.dtype}")
+    dtype, device = query.dtype, query.device
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise NotImplementedError(f"queries must be bfloat16 or float16, not {dtype}")
     tokens, heads, head_size = query.shape
-    if head_size != cache.head_size or heads == 0 or heads % cache.num_heads:
-        raise ValueError(f"query {tuple(query.shape)} does not fit {cache.num_heads} KV heads of {cache.head_size}")
-    if query.stride(2) != 1:
+    codes = cache.codes
+    _, num_blocks, kv_heads, rows, half = codes.shape
+    if head_size != 2 * half or heads == 0 or heads % kv_heads:
+        raise ValueError(f"query {tuple(query.shape)} does not fit {kv_heads} KV heads of {2 * half}")
+    token, head, value = query.stride()
+    if value != 1:
         raise ValueError("query heads must be contiguous")
-    device = query.device
-    if cache.device != device:
+    if codes.device != device:
         raise ValueError("query and cache must live on one device")
     _int32("block_table", block_table, device, 2)
     _int32("seq_lens", seq_lens, device, 1)
-    seqs = seq_lens.shape[0]
-    if block_table.shape[0] != seqs:
+    seqs, width = block_table.shape
+    if seq_lens.shape[0] != seqs:
         raise ValueError("block_table must hold one row per sequence")
+    start = 0
     if query_start is not None:
         _int32("query_start", query_start, device, 1)
         if query_start.shape[0] != seqs + 1:
             raise ValueError("query_start must hold one entry per sequence and one more")
+        start = query_start.data_ptr()
     elif tokens != seqs:
         raise ValueError(f"{tokens} query tokens for {seqs} sequences need query_start")
-    _native.require_cuda(query)
+    if not query.is_cuda:
+        _native.require_cuda(query)
     with on_device(device, stream):
         result = _attention_out(query, out)
         if tokens == 0 or seqs == 0:
             return result
-        need = paged_attention4_workspace_bytes(tokens, seqs, heads, cache.num_heads, head_size)
         if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+            workspace = torch.empty(paged_attention4_workspace_bytes(tokens, seqs, heads, kv_heads, head_size),
+                                    dtype=torch.uint8, device=device)
         elif workspace.dtype != torch.uint8 or workspace.device != device or not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous uint8 on the query's device")
-        token, row, _ = query.stride()
-        out_token, out_row, _ = result.stride()
+        out_token, out_head, _ = result.stride()
         _native.call(
-            "cb_paged_attention4", query.data_ptr(), 2 * token, 2 * row, tokens, heads,
-            _native.DTYPE_CODES[query.dtype], 0 if query_start is None else query_start.data_ptr(), *cache._pages(),
-            cache.num_blocks, cache.block_size, cache.num_heads, head_size,
-            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), seqs, float(scale),
-            result.data_ptr(), 2 * out_token, 2 * out_row, workspace.data_ptr(), workspace.numel(), current_handle())
+            "cb_paged_attention4", query.data_ptr(), 2 * token, 2 * head, tokens, heads, _native.DTYPE_CODES[dtype], start,
+            *cache._pages(), num_blocks, rows, kv_heads, head_size, block_table.data_ptr(), block_table.stride(0), width,
+            seq_lens.data_ptr(), seqs, float(scale), result.data_ptr(), 2 * out_token, 2 * out_head, workspace.data_ptr(),
+            workspace.numel(), current_handle())
         return result
 
 
