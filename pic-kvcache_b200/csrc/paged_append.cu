@@ -12,8 +12,8 @@
 // 4-bit rows: every 64 values of a row share a lowest value and a step,
 //   low = fp16(min x), step = fp16((max x - low') / 15)   (low' = the fp32 minimum)
 //   code = clamp(rint((x - low) * (1 / step)), 0, 15),  value = low + step code
-// fp16 (11 bits) rather than bf16 for the pair: its rounding is 2^-12 of the
-// lowest value, far below a step, where bf16's 2^-9 can exceed one in a channel
+// fp16 (11 bits) rather than bf16 for the pair: its rounding is 2^-11 of the
+// lowest value, far below a step, where bf16's 2^-8 can exceed one in a channel
 // with a large offset.  Values beyond fp16's range are held at +-65504; a group
 // with a NaN or an infinity gets a NaN step, so it reads as NaN.  Two codes to
 // a byte, the lower dimension in the low nibble.

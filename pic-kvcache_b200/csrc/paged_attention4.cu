@@ -27,8 +27,8 @@
 //     lie with q's group sums in three fp16 limbs.
 //   * V: the dimensions are the M rows, the keys the K steps, P the B operand; a
 //     transposing ldmatrix of 16-bit units (four codes of a key) pairs the same
-//     codes of two keys.  P step'_G is rounded to fp16 (11 bits: 2^-12 relative,
-//     against the 2^-9 of a bf16 output) once per group and transposed by
+//     codes of two keys.  P step'_G is rounded to fp16 (11 bits: 2^-11 relative,
+//     against the 2^-8 of a bf16 output) once per group and transposed by
 //     movmatrix.  The roundings weigh with codes less 8, not with codes: 8 times the
 //     sum of the rounded factors (one more product, of ones) is taken off again and
 //     the low terms are taken at code 8, so that a row's offset does not multiply them

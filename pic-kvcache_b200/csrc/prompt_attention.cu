@@ -6,7 +6,7 @@
 // before k - n + j of its own sequence:
 //   out = softmax(scale q k^T over the seen keys) v,  head h on KV head h / groups
 // Logits, softmax and sums are fp32; the unnormalized probabilities are rounded
-// to the element type for the second product (2^-9 bf16, 2^-12 fp16, relative,
+// to the element type for the second product (2^-8 bf16, 2^-11 fp16, relative,
 // each its own: about what rounding the output costs), and O is divided by the
 // fp32 row sum at the end.
 //
