@@ -234,7 +234,8 @@ def append_paged_kv(
     head strides (slices of one projection's output will do).  ``kv_layer``: one of the paged
     layouts of ``scatter_paged_kv`` with rows of ``[kv_heads, head_size]``.  ``slot_mapping``:
     the slot of each token; a NEGATIVE slot marks padding, whose row is not written (unlike
-    ``scatter_paged_kv``, where it wraps).  The slots of one call must be distinct.
+    ``scatter_paged_kv``, where it wraps).  The slots of one call must be distinct, and the rows
+    must not lie in the pages themselves.
     ``rotary_emb``: what carries ``cos_sin_cache`` (float32 or the keys' type), ``head_size``,
     ``rotary_dim`` and ``is_neox_style``; None writes the keys as they are.  Returns
     ``query`` ``[tokens, q_heads, head_size]`` rotated at the same positions, in a new tensor,

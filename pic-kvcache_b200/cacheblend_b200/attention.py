@@ -277,7 +277,11 @@ def prompt_attention(
             workspace = torch.empty(need, dtype=torch.uint8, device=device)
         elif workspace.dtype != torch.uint8 or workspace.device != device or not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous uint8 on the query's device")
-        strides = [2 * s for t in (query, key, value, result) for s in t.stride()[:2]]
+        strides = []
+        for t in (query, key, value, result):  # (a dimension of one entry may carry any stride)
+            token, head, _ = t.stride()
+            head = head if t.shape[1] > 1 else head_size
+            strides += (2 * (token if t.shape[0] > 1 else head * t.shape[1]), 2 * head)
         _native.call(
             "cb_prompt_attention", query.data_ptr(), strides[0], strides[1], key.data_ptr(), strides[2], strides[3],
             value.data_ptr(), strides[4], strides[5], tokens, keys, heads, kv_heads, head_size,

@@ -83,6 +83,10 @@ CASES = [
     (40, 2, 2, 64, 32, False, 1, torch.float32, torch.float32, 0),
     (9, 3, 3, 1, 0, True, 16, torch.float32, torch.float32, 0),         # heads of one value
     (300, 64, 8, 256, 256, True, 128, torch.bfloat16, torch.float32, 8),
+    # enough tokens for several heads per thread, head counts that four does not divide
+    (3001, 10, 5, 128, 128, True, 16, torch.bfloat16, torch.float32, 0),
+    (5003, 7, 7, 64, 32, False, 16, torch.float16, torch.float32, 0),
+    (4001, 6, 3, 128, 32, True, 32, torch.float32, torch.float32, 0),
 ]
 
 
@@ -178,8 +182,8 @@ def test_append_host_indices_and_no_tokens(cuda):
 def _held(x: np.ndarray):
     """(codes, step, low) of fp32 rows [..., 64 g] by the kernel's fp32 steps, and in numpy's IEEE arithmetic."""
     x = x.reshape(*x.shape[:-1], -1, 64).astype(np.float32)
-    low = x.min(-1, keepdims=True)
-    step = ((x.max(-1, keepdims=True) - low) * np.float32(1 / 15)).astype(np.float16)
+    low = np.maximum(x.min(-1, keepdims=True), np.float32(-65504))
+    step = ((np.minimum(x.max(-1, keepdims=True), np.float32(65504)) - low) * np.float32(1 / 15)).astype(np.float16)
     low16 = low.astype(np.float16)
     with np.errstate(divide="ignore"):
         inverse = np.where(step > 0, np.float32(1) / step.astype(np.float32), np.float32(0))
@@ -189,7 +193,8 @@ def _held(x: np.ndarray):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("tokens,kv_heads,head,rotary,neox,block,pad", [
-    (1, 1, 64, 64, True, 16, 0), (50, 3, 128, 128, True, 24, 0), (33, 8, 128, 64, False, 16, 0), (7, 2, 128, 24, True, 1, 1)])
+    (1, 1, 64, 64, True, 16, 0), (50, 3, 128, 128, True, 24, 0), (33, 8, 128, 64, False, 16, 0), (7, 2, 128, 24, True, 1, 1),
+    (6007, 3, 128, 128, True, 16, 0), (6007, 5, 128, 64, True, 16, 0), (9001, 5, 64, 32, True, 16, 0), (9001, 5, 64, 64, False, 16, 0)])
 def test_append_4_bit(cuda, dtype, tokens, kv_heads, head, rotary, neox, block, pad):
     rope = _rope(head, rotary, neox, torch.float32, cuda)
     q, k, v, positions = _inputs(cuda, tokens, 2, kv_heads, head, dtype, 9, pad)
@@ -199,6 +204,10 @@ def test_append_4_bit(cuda, dtype, tokens, kv_heads, head, rotary, neox, block, 
         v[4, 0, :5] = 0                  # an outlier beside zeros
         v[4, 0, 5:64] = 0
         v[4, 0, 9] = 7
+        v[5, 0, :60] = 1.5               # beyond fp16's range, where the type goes there: held at its end
+        v[5, 0, 7], v[5, 0, 30] = min(torch.finfo(dtype).max, 1e30), max(torch.finfo(dtype).min, -3e38)
+        v[6, 0, :64] = -min(torch.finfo(dtype).max, 2e8)
+        v[6, 0, 3] = 17.0
     blocks = tokens // block + 2
     slots = _slots(cuda, tokens, blocks * block, 10)
     cache = PagedKV4.allocate(blocks, block, kv_heads, head, cuda)
@@ -220,7 +229,8 @@ def test_append_4_bit(cuda, dtype, tokens, kv_heads, head, rotary, neox, block, 
         assert np.array_equal(got[plane].cpu().numpy(), value)
         step64, low64 = step.astype(np.float64), low.astype(np.float64)
         bound = step64 / 2 + 2.0 ** -11 * (np.abs(low64) + 15 * step64) + 16 * 2.0 ** -25
-        off = np.abs(value.reshape(codes.shape) - x.double().cpu().numpy().reshape(codes.shape))
+        held = x.double().cpu().numpy().reshape(codes.shape).clip(-65504, 65504)
+        off = np.abs(value.reshape(codes.shape) - held)
         assert (off <= bound * (1 + 1e-5)).all()
     rest = torch.ones(blocks * block, dtype=torch.bool, device=cuda)
     rest[slots] = False

@@ -179,6 +179,45 @@ def test_not_finite(cuda):
     assert bool(got[0, 1].isnan().all()) and bool(got[0, 0].isfinite().all()) and bool(got[1].isfinite().all())
 
 
+@pytest.mark.parametrize("scale", [-0.07, 0.0])
+def test_scales_that_are_not_positive(cuda, scale):
+    lens = [300, 41]
+    cache, table = _pages(cuda, lens, 16, 2, 128, 21)
+    query = torch.randn(2, 8, 128, device=cuda, generator=torch.Generator(device=cuda).manual_seed(1)).to(torch.bfloat16)
+    got = paged_attention4(query, cache, table, torch.tensor(lens, dtype=torch.int32, device=cuda), scale)
+    _check(got, query, cache, table, lens, scale)
+
+
+def test_empty_cache_and_no_sequences(cuda):
+    """No pages at all: every sequence is empty."""
+    empty = PagedKV4(torch.zeros(2, 0, 2, 16, 64, dtype=torch.uint8, device=cuda),
+                     torch.zeros(2, 0, 2, 16, 2, 2, dtype=torch.float16, device=cuda))
+    query = torch.randn(2, 8, 128, device=cuda).to(torch.bfloat16)
+    table, lens = torch.zeros(2, 3, dtype=torch.int32, device=cuda), torch.tensor([20, 0], dtype=torch.int32, device=cuda)
+    cache, _ = _pages(cuda, [20], 16, 2, 128, 1)
+    with pytest.raises(ValueError, match="null page"):
+        paged_attention4(query, empty, table, lens, 0.1)
+    none = torch.full_like(table, cache.num_blocks)  # every page outside the cache
+    assert int((paged_attention4(query, cache, none, lens, 0.1) != 0).sum()) == 0
+    assert int((paged_attention4(query, cache, table[:, :0], lens, 0.1) != 0).sum()) == 0
+    assert paged_attention4(query[:0], cache, table[:0], lens[:0], 0.1).shape == (0, 8, 128)
+
+
+def test_calls_at_once_and_again(cuda):
+    """Calls of different shapes on two streams at once, many times: always the same bits."""
+    problems = []
+    for seed, (lens, heads, kv_heads, head) in enumerate([([5000, 3, 900], 16, 2, 128), ([40] * 90, 8, 4, 64), ([12000], 8, 1, 128)]):
+        cache, table = _pages(cuda, lens, 16, kv_heads, head, seed)
+        query = torch.randn(len(lens), heads, head, device=cuda, generator=torch.Generator(device=cuda).manual_seed(seed)).to(torch.bfloat16)
+        problems.append((query, cache, table, torch.tensor(lens, dtype=torch.int32, device=cuda), 0.1))
+    want = [paged_attention4(*p) for p in problems]
+    torch.cuda.synchronize()
+    sides = [torch.cuda.Stream(cuda) for _ in range(2)]
+    got = [(i, paged_attention4(*problems[i], stream=sides[n % 2])) for n in range(30) for i in range(3)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want[i]) for i, out in got)
+
+
 def test_many_sequences(cuda):
     """More sequences than threads of a CTA, most of them empty or short."""
     gen = torch.Generator().manual_seed(10)

@@ -210,6 +210,30 @@ def test_streams_workspace_and_graph(cuda):
     _check(inside, q, k, v, [0, 400, 500], [0, 400, 500], 0.1)
 
 
+def test_dimensions_of_one(cuda):
+    """One token, one head: whatever strides such dimensions carry."""
+    q, k, v = _inputs(cuda, 1, 1, 1, 1, 64, torch.bfloat16, 9)
+    odd = [torch.as_strided(t, (1, 1, 64), (3, 7, 1)) for t in (q, k, v)]
+    got = prompt_attention(*odd, _starts([1], cuda), 0.1)
+    assert torch.equal(got, v)
+
+
+def test_calls_at_once_and_again(cuda):
+    """Calls of different shapes on two streams at once, many times: always the same bits."""
+    problems = []
+    for seed, (lengths, heads, kv_heads, head) in enumerate([([700, 3, 2100], 16, 2, 128), ([40] * 30, 8, 4, 64), ([900], 14, 2, 128)]):
+        q, k, v = _inputs(cuda, sum(lengths), sum(lengths), heads, kv_heads, head, torch.bfloat16, seed)
+        problems.append((q, k, v, _starts(lengths, cuda), 0.1))
+    want = [prompt_attention(*p) for p in problems]
+    torch.cuda.synchronize()
+    sides = [torch.cuda.Stream(cuda) for _ in range(2)]
+    error = torch.zeros(1, dtype=torch.int32, device=cuda)
+    torch.cuda.synchronize()
+    got = [(i, prompt_attention(*problems[i], stream=sides[n % 2], device_error=error)) for n in range(20) for i in range(3)]
+    torch.cuda.synchronize()
+    assert int(error) == 0 and all(torch.equal(out, want[i]) for i, out in got)
+
+
 def test_long_prompt(cuda):
     """A prompt of many tiles per row, checked on its last rows."""
     q, k, v = _inputs(cuda, 9000, 9000, 4, 1, 128, torch.bfloat16, 8)
