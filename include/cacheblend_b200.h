@@ -508,7 +508,7 @@ CB_API int cb_gather_paged_kv4(const void* k_codes, const void* v_codes, int64_t
  * and pages outside the cache are left out; a row that sees no key is zeros;
  * rows of no sequence are not written; query_start is clamped to the rows there
  * are.  Logits, softmax and sums in fp32, the weighted steps of the values
- * rounded to fp16 before the product with their codes.  `workspace`: 16-byte
+ * rounded to fp16 before the product with their codes.  `workspace`: 32-byte
  * aligned device memory of cb_paged_attention4_workspace_size bytes, any
  * contents; calls that share one must not overlap on the GPU.
  */

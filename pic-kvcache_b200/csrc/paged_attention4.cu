@@ -48,7 +48,7 @@
 // its rounds (a tile per warp) and a fixed cost, cut into equal shares, one per
 // CTA, whatever the lengths are; the cut is found on the device from the lengths.
 // Without the fixed cost the CTAs that got many short sequences ran twice as long
-// as the rest (64 sequences of 1 to 8,192 keys: 130 us).  The first and last piece of a share may be
+// as the rest (64 sequences of 1 to 8,192 keys: 130 us against 74 then).  The first and last piece of a share may be
 // parts; parts go to the workspace and a second launch joins them in order, so a
 // result does not depend on timing.
 #include <algorithm>
@@ -68,13 +68,19 @@ constexpr int kCtas = 2 * kSmCount;
 constexpr int kRound = kWarps;   // tiles of a CTA's round: one per warp
 // What a piece costs besides its rounds, in rounds: its first loads, the query operands and
 // the warps' meeting.
-constexpr int kPieceCost = 2;
+constexpr int kPieceCost = 3;
 // Tables of at most this many keys are not cut: the join's launch costs more than the rounds
 // that a second CTA would take over.
 constexpr int kUncutKeys = 2 * kRound * kTileKeys;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSetRoom = 10.0f;   // a factor p step' is at most 2^10 when M is set,
 constexpr float kMostRoom = 15.0f;  // and 2^15 before M moves
+
+// A piece that a CTA began and others go on with.
+struct alignas(32) Cut {
+  int followers;  // CTAs that go on; negative: no such piece
+  int head, row0, rows, first_token;  // rows: of the sequence and KV head
+};
 
 struct Params {
   const char* query;
@@ -99,7 +105,7 @@ struct Params {
   bool aligned;      // query rows in whole 16-byte vectors
   bool uncut;        // every piece whole in one CTA: nothing to join
   float* parts;      // [ctas][2][rows][D + 2]
-  int4* meta;        // [ctas]: (parts that follow, sequence, KV head, row block); x < 0: none
+  Cut* meta;         // [ctas]
 };
 
 // One sequence's share of the line.
@@ -233,7 +239,7 @@ __device__ __noinline__ void next_piece(const Params& c, Walk& walk, Piece& piec
       continue;
     }
     const int length = s.rounds + kPieceCost;  // a piece's place on the line: its cost, then its rounds
-    const int number = static_cast<int>(walk.offset / length);
+    const int number = (walk.offset >> 31) == 0 ? static_cast<int>(walk.offset) / length : static_cast<int>(walk.offset / length);
     const int from = static_cast<int>(walk.offset - static_cast<int64_t>(number) * length);
     // uncut pieces belong to the share that they begin in
     const int to = c.uncut ? length : static_cast<int>(min(static_cast<int64_t>(length), from + (walk.end - walk.at)));
@@ -249,8 +255,8 @@ __device__ __noinline__ void next_piece(const Params& c, Walk& walk, Piece& piec
     piece.len = s.len, piece.tokens = s.tokens, piece.first_token = s.first_token;
     piece.whole = piece.tile0 == 0 && piece.tile1 == s.tiles;
     if (piece.tile0 == 0 && !piece.whole)
-      c.meta[blockIdx.x] =
-          make_int4(static_cast<int>((length - to + walk.share - 1) / walk.share), walk.seq, piece.head, piece.row0);
+      c.meta[blockIdx.x] = Cut{static_cast<int>((length - to + walk.share - 1) / walk.share), piece.head, piece.row0,
+                               s.tokens * c.groups, s.first_token};
     return;
   }
 }
@@ -292,8 +298,10 @@ __global__ void __launch_bounds__(kThreads, 2) attention4_kernel(const __grid_co
     }
     before += base - mine;  // the line before this thread's sequences
     const int64_t share = (total + gridDim.x - 1) / gridDim.x, begin = share * blockIdx.x;
-    if (threadIdx.x == 0) c.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
-    if (begin >= total) return;
+    if (begin >= total) {
+      if (threadIdx.x == 0) c.meta[blockIdx.x].followers = -1;
+      return;
+    }
     if (before <= begin && begin < before + mine) {
       int64_t left = begin - before;
       int i = lo;
@@ -302,15 +310,19 @@ __global__ void __launch_bounds__(kThreads, 2) attention4_kernel(const __grid_co
         if (left < work) break;
         left -= work;
       }
+      c.meta[blockIdx.x].followers = -1;  // until a cut piece replaces it
       walk = Walk{begin, min(begin + share, total), left, share, i};
+      next_piece(c, walk, piece);
     }
   }
   const uint32_t ring_at = smem_u32(dyn) + warp * kStages * L::kBytes;
 
-  for (;;) {
-    __syncthreads();  // the walk's start is known; the ring and the row values may be written again
-    if (threadIdx.x == 0) next_piece(c, walk, piece);
-    __syncthreads();
+  for (bool first = true;; first = false) {
+    __syncthreads();  // the first piece is known; the ring and the row values may be written again
+    if (!first) {
+      if (threadIdx.x == 0) next_piece(c, walk, piece);
+      __syncthreads();
+    }
     const int tile0 = piece.tile0, tile1 = piece.tile1;
     if (tile1 < 0) break;
     const int head = piece.head, row0 = piece.row0;
@@ -691,31 +703,44 @@ template <int D, typename QT>
 __global__ void __launch_bounds__(kThreads) join4_kernel(const Params c) {
   constexpr int kPer = D / 32;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the parts are still written
-  const int4 meta = c.meta[blockIdx.x];
-  if (meta.x < 0) return;
-  const Seq s = sequence(c, meta.y);
-  const int row = blockIdx.y, r = meta.w + row;
-  if (r >= s.tokens * c.groups) return;
+  const Cut cut = c.meta[blockIdx.x];
+  if (cut.followers < 0) return;
+  const int row = blockIdx.y, r = cut.row0 + row;
+  if (r >= cut.rows) return;
   __shared__ float tops[kWarps], sums[kWarps], values[kWarps][D];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  auto part_of = [&](int i) -> const float* {
-    return c.parts + ((static_cast<int64_t>(blockIdx.x) + i) * 2 + (i == 0)) * kRows * (D + 2) + row * (D + 2);
+  const float* const mine = c.parts + (static_cast<int64_t>(blockIdx.x) * 2 + 1) * kRows * (D + 2) + row * (D + 2);
+  auto part_of = [&](int i) -> const float* {  // part 1 of this CTA, part 0 of the i-th after it
+    return mine + (i == 0 ? int64_t(0) : (2 * static_cast<int64_t>(i) - 1) * kRows * (D + 2));
   };
   float top = -INFINITY, sum = 0.0f, value[kPer];
 #pragma unroll
   for (int j = 0; j < kPer; ++j) value[j] = 0.0f;
-  for (int i = warp; i <= meta.x; i += kWarps) {
-    const float* p = part_of(i);
-    const float pm = p[0], pl = p[1];
-    float v[kPer];
+  constexpr int kAtOnce = 4;  // parts whose loads are in flight together
+  for (int i0 = warp; i0 <= cut.followers; i0 += kAtOnce * kWarps) {
+    float pm[kAtOnce], pl[kAtOnce], v[kAtOnce][kPer];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) v[j] = p[2 + j * 32 + lane];
-    const float now = fmaxf(top, pm);
-    const float keep = top == -INFINITY ? 0.0f : ex2(top - now), by = pm == -INFINITY ? 0.0f : ex2(pm - now);
-    top = now;
-    sum = sum * keep + pl * by;
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int i = i0 + u * kWarps;
+      pm[u] = -INFINITY, pl[u] = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) value[j] = value[j] * keep + v[j] * by;
+      for (int j = 0; j < kPer; ++j) v[u][j] = 0.0f;
+      if (i <= cut.followers) {
+        const float* p = part_of(i);
+        pm[u] = p[0], pl[u] = p[1];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) v[u][j] = p[2 + j * 32 + lane];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const float now = fmaxf(top, pm[u]);
+      const float keep = top == -INFINITY ? 0.0f : ex2(top - now), by = pm[u] == -INFINITY ? 0.0f : ex2(pm[u] - now);
+      top = now;
+      sum = sum * keep + pl[u] * by;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) value[j] = value[j] * keep + v[u][j] * by;
+    }
   }
   if (lane == 0) tops[warp] = top, sums[warp] = sum;
 #pragma unroll
@@ -733,20 +758,22 @@ __global__ void __launch_bounds__(kThreads) join4_kernel(const Params c) {
       v = fmaf(values[u][d], by, v);
     }
     const int token = r / c.groups;
-    QT* dst = reinterpret_cast<QT*>(c.out + (s.first_token + static_cast<int64_t>(token)) * c.out_ts +
-                                    static_cast<int64_t>(meta.z * c.groups + r - token * c.groups) * c.out_hs) + d;
+    QT* dst = reinterpret_cast<QT*>(c.out + (cut.first_token + static_cast<int64_t>(token)) * c.out_ts +
+                                    static_cast<int64_t>(cut.head * c.groups + r - token * c.groups) * c.out_hs) + d;
     *dst = Elem<QT>::from_f(l == 0.0f ? 0.0f : v / l);
   }
 }
 
 // ---------------------------------------------------------------- host side
-constexpr size_t kMetaBytes = (kCtas * sizeof(int4) + 255) / 256 * 256;
+constexpr size_t kMetaBytes = (kCtas * sizeof(Cut) + 255) / 256 * 256;
 size_t workspace(int64_t head_size) {
   return kMetaBytes + static_cast<size_t>(kCtas) * 2 * kRows * (head_size + 2) * sizeof(float);
 }
 
 template <int D, typename QT>
 int launch(const Params& c, cudaStream_t s) {
+  // rows that a piece can have: a group's, where each sequence has one token
+  const int rows = c.start == nullptr ? std::min(kRows, c.groups) : kRows;
   constexpr size_t kBytes = smem_bytes<D>();
   int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(attention4_kernel<D, QT>), kBytes);
   if (rc != CB_OK) return rc;
@@ -755,7 +782,7 @@ int launch(const Params& c, cudaStream_t s) {
   if (rc != CB_OK) return rc;
   if (c.uncut) return CB_OK;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(kCtas, kRows), config.blockDim = dim3(kThreads), config.stream = s;
+  config.gridDim = dim3(kCtas, rows), config.blockDim = dim3(kThreads), config.stream = s;
   cudaLaunchAttribute attribute;  // the join's CTAs may come up before the parts are there; they wait
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute.val.programmaticStreamSerializationAllowed = 1;
@@ -833,7 +860,7 @@ extern "C" int cb_paged_attention4(const void* query, int64_t query_token_stride
   CB_REQUIRE(((rows | reinterpret_cast<uint64_t>(out) | (uint64_t)out_token_stride | (uint64_t)out_head_stride) & 1u) == 0,
              "rows must be aligned to their element size");
   const int64_t groups = num_q_heads / num_kv_heads;
-  CB_REQUIRE((reinterpret_cast<uint64_t>(workspace) & 15u) == 0, "the workspace must be 16-byte aligned");
+  CB_REQUIRE((reinterpret_cast<uint64_t>(workspace) & 31u) == 0, "the workspace must be 32-byte aligned");
   CB_REQUIRE(workspace_bytes >= static_cast<int64_t>(att4::workspace(head_size)), "workspace too small (%lld < %zu)",
              (long long)workspace_bytes, att4::workspace(head_size));
   att4::Params c{};
@@ -865,7 +892,7 @@ extern "C" int cb_paged_attention4(const void* query, int64_t query_token_stride
   c.scale_log2 = scale * att4::kLog2e;
   c.aligned = (rows & 15u) == 0;
   c.uncut = c.width * block_size <= att4::kUncutKeys;
-  c.meta = static_cast<int4*>(workspace);
+  c.meta = static_cast<att4::Cut*>(workspace);
   c.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + att4::kMetaBytes);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return dtype == CB_DTYPE_BF16 ? att4::dispatch<__nv_bfloat16>(c, head_size, s) : att4::dispatch<__half>(c, head_size, s);

@@ -258,7 +258,7 @@ def test_streams_workspace_and_graph(cuda):
     dirty = torch.full((size,), 255, dtype=torch.uint8, device=cuda)
     assert torch.equal(paged_attention4(query, cache, table, lengths, 0.1, workspace=dirty), want)
     with pytest.raises(ValueError, match="workspace"):
-        paged_attention4(query, cache, table, lengths, 0.1, workspace=dirty[:size - 16])
+        paged_attention4(query, cache, table, lengths, 0.1, workspace=dirty[:size - 32])
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         inside = paged_attention4(query, cache, table, lengths, 0.1)
