@@ -7,6 +7,8 @@
 
 #include <cuda.h>  // CUtensorMap types; the encoder is fetched through the runtime
 
+#include <atomic>
+
 #include "cb_common.cuh"
 
 namespace cb {
@@ -267,12 +269,17 @@ using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, 
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 inline int get_encoder(EncodeTiled* fn) {
-  void* ptr = nullptr;
-  cudaDriverEntryPointQueryResult q;
-  cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q);
-  if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || ptr == nullptr) {
-    set_error("cuTensorMapEncodeTiled unavailable: %s", cudaGetErrorString(e));
-    return CB_ERR_CUDA;
+  // the driver's entry point stays the same for the life of the process: looked up once
+  static std::atomic<void*> known{nullptr};
+  void* ptr = known.load(std::memory_order_acquire);
+  if (ptr == nullptr) {
+    cudaDriverEntryPointQueryResult q;
+    cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q);
+    if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || ptr == nullptr) {
+      set_error("cuTensorMapEncodeTiled unavailable: %s", cudaGetErrorString(e));
+      return CB_ERR_CUDA;
+    }
+    known.store(ptr, std::memory_order_release);
   }
   *fn = reinterpret_cast<EncodeTiled>(ptr);
   return CB_OK;

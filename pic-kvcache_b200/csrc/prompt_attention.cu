@@ -74,8 +74,11 @@ struct alignas(16) Item {
 struct Params {
   int kv_heads, groups, tile_queries;  // queries per tile: 128 / groups
   float scale_log2;                    // scale * log2(e)
-  const Item* items;
+  const Item* items;  // null: one sequence, whose items are found from its starts
   const int* num_items;
+  const int32_t* query_start;  // of the one sequence
+  const int32_t* key_start;
+  int num_queries, num_keys;
   const char* value;  // for the epilogue of items with values that are not finite
   int64_t value_ts, value_hs;
   char* out;
@@ -92,6 +95,8 @@ struct Shared {
   uint64_t drain;
   uint32_t tmem_base;
   int abort;
+  Item one;   // the one sequence: its rows, all its queries, the last key its first query sees
+  int items;  // pairs of query tiles of all sequences
   int odd_values;  // a boundary tile held values that are not finite (stays set)
 };
 
@@ -106,9 +111,19 @@ __device__ __forceinline__ int cta_item(int k) {
   const int g = static_cast<int>(gridDim.x), c = static_cast<int>(blockIdx.x);
   return k * g + ((k & 1) ? g - 1 - c : c);
 }
-__device__ __forceinline__ Item load_item(const Params& c, int item) {
-  const int4 v = *reinterpret_cast<const int4*>(c.items + item / c.kv_heads);
+__device__ __forceinline__ Item load_item(const Params& c, const Shared& sh, int item) {
+  const int pair = item / c.kv_heads;
+  if (c.items == nullptr) {  // the last queries have the most keys
+    const int first = (sh.items - 1 - pair) * kPair * c.tile_queries;
+    return Item{sh.one.q_row + first, min(sh.one.queries - first, kPair * c.tile_queries), sh.one.k_row, sh.one.pos + first};
+  }
+  const int4 v = *reinterpret_cast<const int4*>(c.items + pair);
   return Item{v.x, v.y, v.z, v.w};
+}
+// A sequence's rows: starts are clamped to the rows there are.
+__device__ __forceinline__ void span(const int32_t* start, int i, int most, int& first, int& length) {
+  first = min(max(start[i], 0), most);
+  length = min(max(start[i + 1], first), most) - first;
 }
 // Valid queries of tile x of an item, and its key tiles: up to the last key its last query sees.
 __device__ __forceinline__ int tile_valid(const Params& c, const Item& w, int x) {
@@ -226,11 +241,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  if (threadIdx.x == 64) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the list of items is there
+    if (c.items == nullptr) {
+      int queries, keys;
+      span(c.query_start, 0, c.num_queries, sh.one.q_row, queries);
+      span(c.key_start, 0, c.num_keys, sh.one.k_row, keys);
+      sh.one.queries = queries, sh.one.pos = keys - queries;
+      sh.items = (queries + kPair * c.tile_queries - 1) / (kPair * c.tile_queries);
+    } else {
+      sh.items = *c.num_items;
+    }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the list of items is there
-  const int items = *c.num_items * c.kv_heads;
+  const int items = sh.items * c.kv_heads;
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
@@ -243,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int q_armed = -1;
         bool ok = true;
         for (int k = 0, item = cta_item(0); item < items && ok && !aborted(sh); item = cta_item(++k)) {
-          const Item w = load_item(c, item);
+          const Item w = load_item(c, sh, item);
           const int h = item % c.kv_heads;
           const int tiles = max(tile_count(c, w, 0), tile_count(c, w, 1));
           if (tiles == 0) continue;
@@ -316,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       int held = -1, held_from = 0;  // the tile loaded last, where it is not handed on yet
       for (int k = 0, item = cta_item(0); item < items && ok && !aborted(sh); item = cta_item(++k)) {
-        const Item w = load_item(c, item);
+        const Item w = load_item(c, sh, item);
         const int h = item % c.kv_heads;
         const int tiles = max(tile_count(c, w, 0), tile_count(c, w, 1));
         for (int kt = 0; kt < tiles && ok; ++kt, ++t) {
@@ -371,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (++ks == kKStages) ks = 0, kp ^= 1;
         };
         for (int k = 0, item = cta_item(0); item < items && ok && !aborted(sh); item = cta_item(++k)) {
-          const Item w = load_item(c, item);
+          const Item w = load_item(c, sh, item);
           const int n[kPair] = {tile_count(c, w, 0), tile_count(c, w, 1)};
           const int tiles = max(n[0], n[1]);
           if (tiles == 0) continue;
@@ -458,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int t = 0, o_count = 0, tiles_before = 0;
     bool ok = true;
     for (int k = 0, item = cta_item(0); item < items && ok; item = cta_item(++k)) {
-      const Item w = load_item(c, item);
+      const Item w = load_item(c, sh, item);
       const int h = item % c.kv_heads;
       const int n = tile_count(c, w, x), n_b = tile_count(c, w, 1);
       auto last_reader = [&](int kt) { return x == 1 || kt >= n_b; };
@@ -627,11 +653,6 @@ __global__ void __launch_bounds__(kListThreads) list_kernel(const int32_t* __res
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the products' CTAs set themselves up meanwhile
   for (int b = threadIdx.x; b < kBuckets; b += kListThreads) count[b] = 0;
   __syncthreads();
-  // starts are clamped to the rows there are
-  auto span = [](const int32_t* start, int i, int most, int& first, int& length) {
-    first = min(max(start[i], 0), most);
-    length = min(max(start[i + 1], first), most) - first;
-  };
   for (int pass = 0; pass < 2; ++pass) {
     for (int i = warp; i < num_seqs; i += kListThreads / 32) {
       int q0, qn, k0, kn;
@@ -714,8 +735,13 @@ int launch(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap
   constexpr size_t kBytes = smem_bytes<D>();
   const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(prompt_kernel<T, D>), kBytes);
   if (rc != CB_OK) return rc;
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(items * c.kv_heads, kSmCount)));
+  if (c.items == nullptr) {
+    prompt_kernel<T, D><<<grid, kThreads, kBytes, s>>>(q_map, k_map, v_map, c);
+    return launch_status("cb_prompt_attention");
+  }
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(items * c.kv_heads, kSmCount)));
+  config.gridDim = grid;
   config.blockDim = dim3(kThreads), config.dynamicSmemBytes = kBytes, config.stream = s;
   cudaLaunchAttribute attribute;
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -797,17 +823,23 @@ extern "C" int cb_prompt_attention(const void* query, int64_t query_token_stride
   prompt::Params c{};
   c.kv_heads = static_cast<int>(num_kv_heads), c.groups = static_cast<int>(groups), c.tile_queries = tile_queries;
   c.scale_log2 = scale * prompt::kLog2e;
-  int* num_items = static_cast<int*>(workspace);
-  prompt::Item* list = reinterpret_cast<prompt::Item*>(static_cast<char*>(workspace) + 256);
-  c.items = list, c.num_items = num_items;
   c.value = static_cast<const char*>(value), c.value_ts = value_token_stride, c.value_hs = value_head_stride;
   c.out = static_cast<char*>(out), c.out_ts = out_token_stride, c.out_hs = out_head_stride;
   c.error = device_error;
-  prompt::list_kernel<<<1, prompt::kListThreads, 0, s>>>(
-      query_start, key_start, static_cast<int>(num_seqs), static_cast<int>(num_queries), static_cast<int>(num_keys),
-      prompt::kPair * tile_queries, static_cast<int>(items), list, num_items);
-  rc = launch_status("cb_prompt_attention (list)");
-  if (rc != CB_OK) return rc;
+  c.query_start = query_start, c.key_start = key_start;
+  c.num_queries = static_cast<int>(num_queries), c.num_keys = static_cast<int>(num_keys);
+  // One sequence's items are an arithmetic series: no list, and one launch less (a 301-token prompt:
+  // 14.4 us with it).
+  if (num_seqs > 1) {
+    int* num_items = static_cast<int*>(workspace);
+    prompt::Item* list = reinterpret_cast<prompt::Item*>(static_cast<char*>(workspace) + 256);
+    c.items = list, c.num_items = num_items;
+    prompt::list_kernel<<<1, prompt::kListThreads, 0, s>>>(query_start, key_start, static_cast<int>(num_seqs), c.num_queries,
+                                                           c.num_keys, prompt::kPair * tile_queries,
+                                                           static_cast<int>(items), list, num_items);
+    rc = launch_status("cb_prompt_attention (list)");
+    if (rc != CB_OK) return rc;
+  }
   if (dtype == CB_DTYPE_BF16)
     return head_size == 128 ? prompt::launch<__nv_bfloat16, 128>(q_map, k_map, v_map, c, items, s)
                             : prompt::launch<__nv_bfloat16, 64>(q_map, k_map, v_map, c, items, s);
