@@ -28,7 +28,7 @@
 namespace cb {
 namespace append {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;  // of a block, at most
 constexpr int kGroup = 64;  // values that share a step
 constexpr float kHalfMax = 65504.0f;
 
@@ -50,22 +50,17 @@ struct Params {
   char* k_scales;  // 4-bit pages: (step, low) pairs
   char* v_scales;
   int64_t scale_block_stride, scale_slot_stride, scale_head_stride;
-  int64_t num_slots, block_size;
+  int64_t num_slots;
+  int block_size;
   const int64_t* slots;
   // thread layout: units of a token, units and tokens per block
-  int units, units_block, tokens_block;
+  int units, units_block, tokens_block, threads;
 };
 
 // slot -> (block, row), with the short division wherever it does.
-__device__ __forceinline__ void split_slot(int64_t slot, int64_t block_size, int64_t& block, int64_t& row) {
-  if ((slot | block_size) >> 31) {
-    block = slot / block_size;
-    row = slot - block * block_size;
-  } else {
-    const uint32_t b = static_cast<uint32_t>(slot) / static_cast<uint32_t>(block_size);
-    block = b;
-    row = static_cast<uint32_t>(slot) - b * static_cast<uint32_t>(block_size);
-  }
+__device__ __forceinline__ void split_slot(int64_t slot, int block_size, int& block, int& row) {
+  block = (slot >> 31) == 0 ? static_cast<int>(slot) / block_size : static_cast<int>(slot / block_size);
+  row = static_cast<int>(slot - static_cast<int64_t>(block) * block_size);
 }
 
 // N consecutive elements as fp32.  WIDE: the address is aligned to the vector.
@@ -183,7 +178,7 @@ __device__ __forceinline__ void rotated(const T* row, int d0, const TAB* table, 
 // Where a thread works: a token, and one piece of HPT heads of K (plane 0), V (1) or Q (2).
 struct Place {
   bool real;
-  int64_t token;
+  int token;  // (32 bits: an address is then one short product and a sum per stride)
   int plane, head, piece;
 };
 template <int HPT, typename P>
@@ -191,7 +186,7 @@ __device__ __forceinline__ Place place(const P& c, int kv_heads, int q_heads, in
   Place w;
   const int tok = threadIdx.x / c.units_block;
   const int unit = blockIdx.y * c.units_block + (threadIdx.x - tok * c.units_block);
-  w.token = static_cast<int64_t>(blockIdx.x) * c.tokens_block + tok;
+  w.token = static_cast<int>(min(static_cast<int64_t>(blockIdx.x) * c.tokens_block + tok, c.tokens));
   w.real = tok < c.tokens_block && unit < c.units && w.token < c.tokens;
   const int bundles = unit / pieces;  // of HPT heads
   const int kv_bundles = (kv_heads + HPT - 1) / HPT;
@@ -205,7 +200,8 @@ __device__ __forceinline__ Place place(const P& c, int kv_heads, int q_heads, in
 struct Target {
   bool turned;  // the position lies inside the table (or nothing is rotated)
   bool stored;  // K or V with a slot of the cache
-  int64_t position, block, row;
+  int64_t position;
+  int block, row;
 };
 __device__ __forceinline__ Target target(const Params& c, const Place& w) {
   Target g{};
@@ -225,7 +221,7 @@ __device__ __forceinline__ Target target(const Params& c, const Place& w) {
 // partners of a rotation, so that each is read once and one piece of the table serves
 // both -- in HPT heads, whose loads are in flight together and share the table's values.
 // HPT 4 at long prompts, 1 where there are too few tokens to fill the GPU (more_heads).
-// A prompt of 16,384 tokens, 32 + 8 + 8 heads of 128: 77 us, 5.3 TB/s; 137 us when the loads
+// A prompt of 16,384 tokens, 32 + 8 + 8 heads of 128: 69 us, 5.9 TB/s; 137 us when the loads
 // waited for slots and positions and each thread had one piece.
 template <typename T, typename TAB, int HPT>
 __global__ void __launch_bounds__(kThreads) append_kernel(const Params c) {
@@ -660,13 +656,14 @@ struct GatherParams {
   const char* v_scales;
   int64_t block_stride, slot_stride, head_stride;
   int64_t scale_block_stride, scale_slot_stride, scale_head_stride;
-  int64_t num_slots, block_size;
+  int64_t num_slots;
+  int block_size;
   int heads, head_size;
   const int64_t* slots;
   int64_t tokens;
   char* out;
   int64_t out_plane_stride, out_token_stride, out_head_stride;
-  int units, units_block, tokens_block;
+  int units, units_block, tokens_block, threads;
 };
 
 // 16 values of HPT heads of K or V per thread; a slot outside the cache reads as zeros.
@@ -681,7 +678,7 @@ __global__ void __launch_bounds__(kThreads) gather4_kernel(const GatherParams c)
 #pragma unroll
   for (int i = 0; i < HPT; ++i) codes[i] = make_uint2(0, 0), pair[i] = make_float2(0.0f, 0.0f);
   if (slot >= 0 && slot < c.num_slots) {
-    int64_t block, row;
+    int block, row;
     split_slot(slot, c.block_size, block, row);
     const char* src = (w.plane ? c.v_codes : c.k_codes) + block * c.block_stride + row * c.slot_stride + d0 / 2;
     const char* sc = (w.plane ? c.v_scales : c.k_scales) + block * c.scale_block_stride + row * c.scale_slot_stride +
@@ -709,12 +706,14 @@ __global__ void __launch_bounds__(kThreads) gather4_kernel(const GatherParams c)
     }
 }
 
-// Threads of a block: the units of one token, or of several tokens side by side.
+// Threads of a block: the units of one token, or of several tokens side by side, and no idle
+// ones behind them (32 + 8 + 8 heads: 96 units, 192 threads; 256 with 64 idle took 77 us, not 69).
 template <typename P>
 dim3 lay_out(P& c, int64_t units, int64_t tokens) {
   c.units = static_cast<int>(units);
   c.units_block = static_cast<int>(std::min<int64_t>(units, kThreads));
   c.tokens_block = kThreads / c.units_block;
+  c.threads = (c.units_block * c.tokens_block + 31) / 32 * 32;
   return dim3(static_cast<unsigned>((tokens + c.tokens_block - 1) / c.tokens_block),
               static_cast<unsigned>((units + c.units_block - 1) / c.units_block));
 }
@@ -740,15 +739,15 @@ void launch4(const Params& c, dim3 grid, bool wide, bool more, cudaStream_t s) {
     const bool extra = c.neox && c.rotary_dim > 0 && c.rotary_dim < D;
     if (wide) {
       if (extra)
-        more ? append4_kernel<T, TAB, D, true, 2><<<grid, kThreads, 0, s>>>(c)
-             : append4_kernel<T, TAB, D, true, 1><<<grid, kThreads, 0, s>>>(c);
+        more ? append4_kernel<T, TAB, D, true, 2><<<grid, c.threads, 0, s>>>(c)
+             : append4_kernel<T, TAB, D, true, 1><<<grid, c.threads, 0, s>>>(c);
       else
-        more ? append4_kernel<T, TAB, D, false, 2><<<grid, kThreads, 0, s>>>(c)
-             : append4_kernel<T, TAB, D, false, 1><<<grid, kThreads, 0, s>>>(c);
+        more ? append4_kernel<T, TAB, D, false, 2><<<grid, c.threads, 0, s>>>(c)
+             : append4_kernel<T, TAB, D, false, 1><<<grid, c.threads, 0, s>>>(c);
       return;
     }
   }
-  append4_narrow_kernel<T, TAB, D><<<grid, kThreads, 0, s>>>(c);
+  append4_narrow_kernel<T, TAB, D><<<grid, c.threads, 0, s>>>(c);
 }
 
 template <bool FOUR, typename T, typename TAB>
@@ -767,11 +766,11 @@ int launch(Params& c, bool wide, cudaStream_t s) {
       launch4<T, TAB, 128>(c, grid, wide, more, s);
   } else {
     if (!wide)
-      append_narrow_kernel<T, TAB><<<grid, kThreads, 0, s>>>(c);
+      append_narrow_kernel<T, TAB><<<grid, c.threads, 0, s>>>(c);
     else if (more)
-      append_kernel<T, TAB, 4><<<grid, kThreads, 0, s>>>(c);
+      append_kernel<T, TAB, 4><<<grid, c.threads, 0, s>>>(c);
     else
-      append_kernel<T, TAB, 1><<<grid, kThreads, 0, s>>>(c);
+      append_kernel<T, TAB, 1><<<grid, c.threads, 0, s>>>(c);
   }
   return launch_status(FOUR ? "cb_append_paged_kv4" : "cb_append_paged_kv");
 }
@@ -795,11 +794,11 @@ void launch_gather4(GatherParams& c, bool wide, cudaStream_t s) {
   const bool four = wide && more_heads(units, c.tokens);
   const dim3 grid = lay_out(c, four ? units_of(c.heads, 0, pieces, 4) : units, c.tokens);
   if (!wide)
-    gather4_kernel<T, false, 1><<<grid, kThreads, 0, s>>>(c);
+    gather4_kernel<T, false, 1><<<grid, c.threads, 0, s>>>(c);
   else if (four)
-    gather4_kernel<T, true, 4><<<grid, kThreads, 0, s>>>(c);
+    gather4_kernel<T, true, 4><<<grid, c.threads, 0, s>>>(c);
   else
-    gather4_kernel<T, true, 1><<<grid, kThreads, 0, s>>>(c);
+    gather4_kernel<T, true, 1><<<grid, c.threads, 0, s>>>(c);
 }
 
 // What both appends check of their rows and of the rotation.
@@ -807,7 +806,7 @@ int check_rows(const Params& c, int dtype, int table_dtype, int64_t num_blocks) 
   CB_SUPPORTED(dtype_bytes(dtype) != 0, "unsupported element type code %d", dtype);
   CB_REQUIRE(c.tokens >= 0 && c.kv_heads > 0 && c.head_size > 0 && num_blocks >= 0 && c.block_size > 0 && c.q_heads >= 0,
              "negative or zero size");
-  CB_REQUIRE(c.tokens < (int64_t(1) << 31) && num_blocks < (int64_t(1) << 40) && c.block_size < (int64_t(1) << 22),
+  CB_REQUIRE(c.tokens < (int64_t(1) << 31) && num_blocks < (int64_t(1) << 31) && c.block_size < (int64_t(1) << 22),
              "size out of range");
   CB_REQUIRE(c.rotary_dim >= 0 && c.rotary_dim <= c.head_size && c.rotary_dim % 2 == 0,
              "rotary_dim %d does not fit the head size %d", c.rotary_dim, c.head_size);
@@ -871,7 +870,9 @@ extern "C" int cb_append_paged_kv(const void* key, int64_t key_token_stride, int
                                   int64_t slot_stride, int64_t head_stride, int64_t num_blocks, int64_t block_size,
                                   const int64_t* slots, void* stream) {
   CB_BIND(stream, k_cache);
-  CB_REQUIRE(num_kv_heads < 65536 && num_q_heads < 65536 && head_size <= 65536 && rotary_dim <= 65536, "size out of range");
+  CB_REQUIRE(num_kv_heads < 65536 && num_q_heads < 65536 && head_size <= 65536 && rotary_dim <= 65536 &&
+                 block_size < (int64_t(1) << 22),
+             "size out of range");
   append::Params c{};
   c.key = static_cast<const char*>(key), c.value = static_cast<const char*>(value);
   c.query = static_cast<const char*>(query), c.query_out = static_cast<char*>(query_out);
@@ -885,7 +886,7 @@ extern "C" int cb_append_paged_kv(const void* key, int64_t key_token_stride, int
   c.rotary_dim = static_cast<int>(rotary_dim), c.neox = is_neox;
   c.k_cache = static_cast<char*>(k_cache), c.v_cache = static_cast<char*>(v_cache);
   c.block_stride = block_stride, c.slot_stride = slot_stride, c.head_stride = head_stride;
-  c.num_slots = num_blocks * block_size, c.block_size = block_size, c.slots = slots;
+  c.num_slots = num_blocks * block_size, c.block_size = static_cast<int>(block_size), c.slots = slots;
   int rc = append::check_rows(c, dtype, cos_sin_dtype, num_blocks);
   if (rc != CB_OK || num_tokens == 0) return rc;
   const uint64_t pages = reinterpret_cast<uint64_t>(k_cache) | reinterpret_cast<uint64_t>(v_cache) | (uint64_t)block_stride |
@@ -907,7 +908,9 @@ extern "C" int cb_append_paged_kv4(const void* key, int64_t key_token_stride, in
                                    int64_t scale_block_stride, int64_t scale_slot_stride, int64_t scale_head_stride,
                                    int64_t num_blocks, int64_t block_size, const int64_t* slots, void* stream) {
   CB_BIND(stream, k_codes);
-  CB_REQUIRE(num_kv_heads < 65536 && num_q_heads < 65536 && head_size <= 65536 && rotary_dim <= 65536, "size out of range");
+  CB_REQUIRE(num_kv_heads < 65536 && num_q_heads < 65536 && head_size <= 65536 && rotary_dim <= 65536 &&
+                 block_size < (int64_t(1) << 22),
+             "size out of range");
   append::Params c{};
   c.key = static_cast<const char*>(key), c.value = static_cast<const char*>(value);
   c.query = static_cast<const char*>(query), c.query_out = static_cast<char*>(query_out);
@@ -924,7 +927,7 @@ extern "C" int cb_append_paged_kv4(const void* key, int64_t key_token_stride, in
   c.k_scales = static_cast<char*>(k_scales), c.v_scales = static_cast<char*>(v_scales);
   c.scale_block_stride = scale_block_stride, c.scale_slot_stride = scale_slot_stride;
   c.scale_head_stride = scale_head_stride;
-  c.num_slots = num_blocks * block_size, c.block_size = block_size, c.slots = slots;
+  c.num_slots = num_blocks * block_size, c.block_size = static_cast<int>(block_size), c.slots = slots;
   int rc = append::check_rows(c, dtype, cos_sin_dtype, num_blocks);
   if (rc != CB_OK || num_tokens == 0) return rc;
   rc = append::check_pages4(block_stride, slot_stride, head_stride, scale_block_stride, scale_slot_stride,
@@ -943,7 +946,7 @@ extern "C" int cb_gather_paged_kv4(const void* k_codes, const void* v_codes, int
   CB_BIND(stream, out);
   CB_SUPPORTED(dtype_bytes(dtype) != 0, "unsupported element type code %d", dtype);
   CB_REQUIRE(num_tokens >= 0 && num_blocks >= 0 && block_size > 0 && num_heads > 0, "negative or zero size");
-  CB_REQUIRE(num_tokens < (int64_t(1) << 31) && num_blocks < (int64_t(1) << 40) && block_size < (int64_t(1) << 22) &&
+  CB_REQUIRE(num_tokens < (int64_t(1) << 31) && num_blocks < (int64_t(1) << 31) && block_size < (int64_t(1) << 22) &&
                  num_heads < 65536,
              "size out of range");
   if (num_tokens == 0) return CB_OK;
@@ -960,7 +963,7 @@ extern "C" int cb_gather_paged_kv4(const void* k_codes, const void* v_codes, int
   c.block_stride = block_stride, c.slot_stride = slot_stride, c.head_stride = head_stride;
   c.scale_block_stride = scale_block_stride, c.scale_slot_stride = scale_slot_stride;
   c.scale_head_stride = scale_head_stride;
-  c.num_slots = num_blocks * block_size, c.block_size = block_size;
+  c.num_slots = num_blocks * block_size, c.block_size = static_cast<int>(block_size);
   c.heads = static_cast<int>(num_heads), c.head_size = static_cast<int>(head_size);
   c.slots = slots, c.tokens = num_tokens, c.out = static_cast<char*>(out);
   c.out_plane_stride = out_plane_stride, c.out_token_stride = out_token_stride, c.out_head_stride = out_head_stride;
