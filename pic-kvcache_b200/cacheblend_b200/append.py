@@ -97,100 +97,107 @@ class PagedKV4:
 
 
 _HERE = contextlib.nullcontext()
+_raw_stream = torch._C._cuda_getCurrentRawStream  # no Stream object is built (2 us of a decode call)
 
 
-def on_device(device: torch.device, stream: torch.cuda.Stream | None):
+def on_device(device: int, stream: torch.cuda.Stream | None):
     """Context in which a call allocates and launches: ``stream``, or the device's current stream."""
     if stream is not None:
-        if stream.device != device:
-            raise ValueError(f"the stream belongs to {stream.device}, the tensors to {device}")
+        if stream.device.index != device:
+            raise ValueError(f"the stream belongs to {stream.device}, the tensors to cuda:{device}")
         return torch.cuda.stream(stream)
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device == torch.cuda.current_device() else torch.cuda.device(device)
 
 
-def current_handle() -> int:
-    """The current device's current stream, without building a Stream object (2 us of a decode call)."""
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+def _contiguous_empty(like: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of ``like``'s shape, type and device."""
+    return torch.empty_like(like) if like.is_contiguous() else torch.empty_like(like, memory_format=torch.contiguous_format)
 
 
-def _index(name: str, index: torch.Tensor, count: int, device: torch.device, low: int | None, high: int) -> torch.Tensor:
+def _index(name: str, index: torch.Tensor, count: int, device: int, low: int | None, high: int) -> torch.Tensor:
     """One int64 per token on ``device``; host values are range-checked first."""
-    if index.ndim != 1 or index.shape[0] != count:
+    if index.ndim != 1 or index.numel() != count:
         raise ValueError(f"{name} must hold one entry per token ({count}), got shape {tuple(index.shape)}")
-    if index.dtype == torch.long and index.device == device:
-        return index if index.is_contiguous() else index.contiguous()
+    where = index.get_device()
+    if where == device and index.dtype is torch.long and index.is_contiguous():
+        return index
     if index.is_floating_point() or index.dtype == torch.bool:
         raise ValueError(f"{name} must be whole numbers, not {index.dtype}")
     if index.device.type == "cpu":
         if count and ((low is not None and int(index.min()) < low) or int(index.max()) >= high):
             raise IndexError(f"{name} out of range: [{int(index.min())}, {int(index.max())}] for {high}")
-    elif index.device != device:
-        raise ValueError(f"{name} must live on the host or on {device}")
-    return index.to(device=device, dtype=torch.long).contiguous()
+    elif where != device:
+        raise ValueError(f"{name} must live on the host or on cuda:{device}")
+    return index.to(device=torch.device("cuda", device), dtype=torch.long).contiguous()
 
 
-def _check_rows(key: torch.Tensor, value: torch.Tensor, query: torch.Tensor | None) -> tuple[int, int, int]:
-    """(tokens, kv_heads, head_size) of rows that go together."""
-    shape, dtype, device = key.shape, key.dtype, key.device
+def _check_rows(key: torch.Tensor, value: torch.Tensor, query: torch.Tensor | None) -> tuple:
+    """(shape, dtype, device index, strides of key, of value, of query) of rows that go together."""
+    shape, dtype, device = key.shape, key.dtype, key.get_device()
     if len(shape) != 3:
         raise ValueError(f"key must be [tokens, heads, head_size], got {tuple(shape)}")
     if value.shape != shape:
         raise ValueError(f"key and value must have the same shape, not {tuple(shape)} and {tuple(value.shape)}")
-    if value.dtype != dtype or value.device != device:
+    if value.dtype is not dtype or value.get_device() != device:
         raise ValueError("value must share the keys' dtype and device")
+    of_key, of_value, of_query = key.stride(), value.stride(), (0, 0, 1)
     if query is not None:
         q = query.shape
         if len(q) != 3 or q[0] != shape[0] or q[2] != shape[2]:
             raise ValueError(f"query {tuple(q)} does not match the keys {tuple(shape)}")
-        if query.dtype != dtype or query.device != device:
+        if query.dtype is not dtype or query.get_device() != device:
             raise ValueError("query must share the keys' dtype and device")
-    if shape[2] > 1 and (key.stride(2) != 1 or value.stride(2) != 1 or (query is not None and query.stride(2) != 1)):
+        of_query = query.stride()
+    if shape[2] > 1 and not (of_key[2] == of_value[2] == of_query[2] == 1):
         raise ValueError("the values of a head must be contiguous in key, value and query")
-    _native.dtype_code(dtype)
-    return shape
+    if dtype not in _native.DTYPE_CODES:
+        _native.dtype_code(dtype)
+    return shape, dtype, device, of_key, of_value, of_query
 
 
 def _page_planes(kv_layer: KVLayer, block_size: int) -> tuple:
-    """(K address, V address, shape, strides, dtype, device) of 16/32-bit pages [blocks, rows, heads, head_size].
+    """(K address, V address, shape, strides, dtype, device index) of 16/32-bit pages [blocks, rows, heads, head_size].
 
     The merged layouts are taken apart by arithmetic: describe_paged's views are most of a
     decode step's call.  Whatever is unusual goes through it."""
     if isinstance(kv_layer, torch.Tensor) and kv_layer.ndim == 5:
         shape, strides = kv_layer.shape, kv_layer.stride()
-        plane = 0 if shape[0] == 2 else 1 if shape[1] == 2 else None
-        if plane is not None and 0 < block_size <= shape[2]:
-            key = kv_layer.data_ptr()
-            return (key, key + strides[plane] * kv_layer.element_size(), (shape[1 - plane], *shape[2:]),
-                    (strides[1 - plane], *strides[2:]), kv_layer.dtype, kv_layer.device)
+        key = kv_layer.data_ptr()
+        if shape[0] == 2 and 0 < block_size <= shape[2]:
+            return (key, key + strides[0] * kv_layer.element_size(), shape[1:], strides[1:], kv_layer.dtype,
+                    kv_layer.get_device())
+        if shape[1] == 2 and shape[0] != 2 and 0 < block_size <= shape[2]:
+            return (key, key + strides[1] * kv_layer.element_size(), (shape[0], *shape[2:]), (strides[0], *strides[2:]),
+                    kv_layer.dtype, kv_layer.get_device())
     paged = describe_paged(kv_layer, block_size)
-    return (paged.key.data_ptr(), paged.value.data_ptr(), tuple(paged.key.shape), paged.key.stride(), paged.dtype,
-            paged.device)
+    return (paged.key.data_ptr(), paged.value.data_ptr(), paged.key.shape, paged.key.stride(), paged.dtype,
+            paged.key.get_device())
 
 
-def _rotation(rotary_emb, head_size: int, key: torch.Tensor) -> tuple:
+def _rotation(rotary_emb, head_size: int, dtype: torch.dtype, device: int) -> tuple:
     """(table or None, table dtype code, positions it holds, rotary_dim, neox)."""
     if rotary_emb is None:
         return None, _native.DTYPE_CODES[torch.float32], 0, 0, 1
     table = rotary_emb.cos_sin_cache
     rotary_dim = int(getattr(rotary_emb, "rotary_dim", head_size))
-    if int(rotary_emb.head_size) != head_size:
+    if rotary_emb.head_size != head_size:
         raise ValueError(f"the rotation is made for heads of {rotary_emb.head_size} values, not {head_size}")
     if table.ndim != 2 or table.shape[1] != rotary_dim or rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError("RoPE cache width does not match rotary_dim")
-    if table.device != key.device:
+    if table.get_device() != device:
         raise ValueError("the RoPE cache must live on the keys' device")
-    if table.dtype not in (torch.float32, key.dtype):
-        raise NotImplementedError(f"the RoPE cache must be float32 or {key.dtype}, not {table.dtype}")
-    return table.contiguous(), _native.dtype_code(table.dtype), int(table.shape[0]), rotary_dim, \
-        int(bool(rotary_emb.is_neox_style))
+    if table.dtype is not torch.float32 and table.dtype is not dtype:
+        raise NotImplementedError(f"the RoPE cache must be float32 or {dtype}, not {table.dtype}")
+    if not table.is_contiguous():
+        table = table.contiguous()
+    return table, _native.DTYPE_CODES[table.dtype], table.shape[0], rotary_dim, 1 if rotary_emb.is_neox_style else 0
 
 
-def _append(entry: str, rotary_emb, positions, key, value, query, slot_mapping, num_blocks: int, block_size: int,
-            pages: tuple, stream) -> torch.Tensor | None:
-    tokens, heads, head_size = key.shape
-    device = key.device
-    table, table_code, max_position, rotary_dim, neox = _rotation(rotary_emb, head_size, key)
+def _append(entry: str, rotary_emb, positions, key, value, query, rows: tuple, slot_mapping, num_blocks: int,
+            block_size: int, pages: tuple, stream) -> torch.Tensor | None:
+    (tokens, heads, head_size), dtype, device, of_key, of_value, of_query = rows
     with on_device(device, stream):
+        table, table_code, max_position, rotary_dim, neox = _rotation(rotary_emb, head_size, dtype, device)
         slots = _index("slot_mapping", slot_mapping, tokens, device, None, num_blocks * block_size)
         where = 0
         if rotary_dim:
@@ -198,22 +205,18 @@ def _append(entry: str, rotary_emb, positions, key, value, query, slot_mapping, 
                 raise ValueError("a rotation needs one position per token")
             positions = _index("positions", positions, tokens, device, 0, max_position)
             where = positions.data_ptr()
-        turned, q_heads, q = None, 0, (0, 0, 0, 0, 0, 0)
+        turned, q_heads, q, out = None, 0, 0, 0
         size = key.element_size()
         if query is not None:
-            turned = torch.empty_like(query, memory_format=torch.contiguous_format)
-            q_heads = query.shape[1]
-            from_token, from_head, _ = query.stride()
-            q = (query.data_ptr(), from_token * size, from_head * size, turned.data_ptr(), q_heads * head_size * size,
-                 head_size * size)
+            turned = _contiguous_empty(query)
+            q_heads, q, out = query.shape[1], query.data_ptr(), turned.data_ptr()
         if tokens == 0:
             return turned
-        key_token, key_head, _ = key.stride()
-        value_token, value_head, _ = value.stride()
-        _native.call(entry, key.data_ptr(), key_token * size, key_head * size, value.data_ptr(), value_token * size,
-                     value_head * size, *q, tokens, q_heads, heads, head_size, _native.DTYPE_CODES[key.dtype], where,
+        _native.call(entry, key.data_ptr(), of_key[0] * size, of_key[1] * size, value.data_ptr(), of_value[0] * size,
+                     of_value[1] * size, q, of_query[0] * size, of_query[1] * size, out, q_heads * head_size * size,
+                     head_size * size, tokens, q_heads, heads, head_size, _native.DTYPE_CODES[dtype], where,
                      0 if table is None else table.data_ptr(), table_code, max_position, rotary_dim, neox, *pages,
-                     num_blocks, block_size, slots.data_ptr(), current_handle())
+                     num_blocks, block_size, slots.data_ptr(), _raw_stream(device))
         return turned
 
 
@@ -246,20 +249,20 @@ def append_paged_kv(
     outside the cache, or a position outside the table, leaves the pages as they were (and
     gives a zero query row).
     """
-    _, heads, head_size = _check_rows(key, value, query)
-    k_pages, v_pages, shape, strides, dtype, device = _page_planes(kv_layer, block_size)
-    if not key.is_cuda or device.type != "cuda":
+    checked = _check_rows(key, value, query)
+    (_, heads, head_size), dtype, device, _, _, _ = checked
+    k_pages, v_pages, shape, strides, cache_dtype, cache_device = _page_planes(kv_layer, block_size)
+    if device < 0 or cache_device < 0:
         _native.require_cuda(key, *(kv_layer if not isinstance(kv_layer, torch.Tensor) else (kv_layer,)))
-    if key.dtype != dtype or key.device != device:
+    if dtype is not cache_dtype or device != cache_device:
         raise ValueError("keys must match the KV cache dtype and device")
     if len(shape) != 4 or shape[2] != heads or shape[3] != head_size:
         raise ValueError(f"pages {tuple(shape)} do not hold rows of {(heads, head_size)}")
-    if head_size > 1 and strides[3] != 1:
+    if strides[3] != 1 and head_size > 1:
         raise ValueError("the values of a head must be contiguous in the pages")
     size = key.element_size()
-    pages = (k_pages, v_pages, strides[0] * size, strides[1] * size, strides[2] * size)
-    return _append("cb_append_paged_kv", rotary_emb, positions, key, value, query, slot_mapping, shape[0], block_size,
-                   pages, stream)
+    return _append("cb_append_paged_kv", rotary_emb, positions, key, value, query, checked, slot_mapping, shape[0],
+                   block_size, (k_pages, v_pages, strides[0] * size, strides[1] * size, strides[2] * size), stream)
 
 
 def append_paged_kv4(
@@ -279,15 +282,16 @@ def append_paged_kv4(
     nearest.  Values beyond +-65504 are held at that; a group with a NaN or an infinity reads
     as NaN.
     """
-    _, heads, head_size = _check_rows(key, value, query)
-    if not key.is_cuda or not cache.codes.is_cuda:
+    checked = _check_rows(key, value, query)
+    (_, heads, head_size), _, device, _, _, _ = checked
+    if device < 0 or not cache.codes.is_cuda:
         _native.require_cuda(cache.codes, key)
-    if key.device != cache.device:
+    if device != cache.codes.get_device():
         raise ValueError("keys must live on the cache's device")
     _, num_blocks, cache_heads, rows, half = cache.codes.shape
     if heads != cache_heads or head_size != 2 * half:
         raise ValueError(f"the cache holds rows of {(cache_heads, 2 * half)}, not {(heads, head_size)}")
-    return _append("cb_append_paged_kv4", rotary_emb, positions, key, value, query, slot_mapping, num_blocks, rows,
+    return _append("cb_append_paged_kv4", rotary_emb, positions, key, value, query, checked, slot_mapping, num_blocks, rows,
                    cache._pages(), stream)
 
 
@@ -303,26 +307,30 @@ def gather_paged_kv4(
     A negative slot (padding) reads as zeros; so does, on the device, one outside the cache
     (IndexError for host slots).
     """
-    if not cache.codes.is_cuda:
-        _native.require_cuda(cache.codes)
-    _, num_blocks, heads, rows, half = cache.codes.shape
-    tokens, device = slot_mapping.numel(), cache.device
+    codes = cache.codes
+    device = codes.get_device()
+    if device < 0:
+        _native.require_cuda(codes)
+    _, num_blocks, heads, rows, half = codes.shape
+    tokens = slot_mapping.numel()
     shape = (2, tokens, heads, 2 * half)
-    code = _native.dtype_code(dtype)
+    if dtype not in _native.DTYPE_CODES:
+        _native.dtype_code(dtype)
     if out is not None:
-        if tuple(out.shape) != shape:
+        if out.shape != shape:
             raise ValueError(f"gather output has shape {tuple(out.shape)}, expected {shape}")
-        if out.dtype != dtype or out.device != device:
+        if out.dtype is not dtype or out.get_device() != device:
             raise ValueError("gather output must match the dtype and the cache's device")
         if out.stride(3) != 1:
             raise ValueError("the values of a head must be contiguous in the output")
     with on_device(device, stream):
         slots = _index("slot_mapping", slot_mapping, tokens, device, None, num_blocks * rows)
-        result = out if out is not None else torch.empty(shape, dtype=dtype, device=device)
+        result = out if out is not None else torch.empty(shape, dtype=dtype, device=codes.device)
         if tokens == 0:
             return result
         size = result.element_size()
         plane, token, head, _ = result.stride()
         _native.call("cb_gather_paged_kv4", *cache._pages(), num_blocks, rows, heads, 2 * half, slots.data_ptr(), tokens,
-                     result.data_ptr(), plane * size, token * size, head * size, code, current_handle())
+                     result.data_ptr(), plane * size, token * size, head * size, _native.DTYPE_CODES[dtype],
+                     _raw_stream(device))
         return result

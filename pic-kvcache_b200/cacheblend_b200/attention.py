@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 from . import _native
-from .append import PagedKV4, current_handle, on_device
+from .append import PagedKV4, _contiguous_empty, _raw_stream, on_device
 
 
 # exact_rounding argument -> the C ABI's mode code
@@ -100,21 +100,33 @@ def blend_attention(
     return out
 
 
-def _int32(name: str, tensor: torch.Tensor, device: torch.device, ndim: int) -> None:
-    if tensor.dtype != torch.int32 or tensor.device != device or tensor.ndim != ndim:
-        raise ValueError(f"{name} must be a {ndim}-dimensional int32 tensor on {device}")
-    if tensor.stride(-1) != 1 and tensor.shape[-1] > 1:
+_HALVES = (torch.bfloat16, torch.float16)
+
+
+def _int32(name: str, tensor: torch.Tensor, device: int, ndim: int) -> None:
+    if tensor.dtype is not torch.int32 or tensor.get_device() != device or tensor.ndim != ndim:
+        raise ValueError(f"{name} must be a {ndim}-dimensional int32 tensor on the query's device")
+    if not tensor.is_contiguous() and tensor.stride(-1) != 1 and tensor.shape[-1] > 1:
         raise ValueError(f"{name} must be contiguous")
 
 
 def _attention_out(query: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
     if out is None:
-        return torch.empty_like(query, memory_format=torch.contiguous_format)
+        return _contiguous_empty(query)
     if out.shape != query.shape or out.dtype != query.dtype or out.device != query.device:
         raise ValueError("out must match the query's shape, dtype and device")
     if out.stride(2) != 1:
         raise ValueError("out heads must be contiguous")
     return out
+
+
+def _scratch(workspace: torch.Tensor | None, need, device: torch.device) -> torch.Tensor:
+    """The caller's workspace, or one of ``need()`` bytes."""
+    if workspace is None:
+        return torch.empty(need(), dtype=torch.uint8, device=device)
+    if workspace.dtype != torch.uint8 or workspace.device != device or not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous uint8 on the query's device")
+    return workspace
 
 
 def paged_attention4_workspace_bytes(num_tokens: int, num_seqs: int, num_q_heads: int, num_kv_heads: int,
@@ -152,49 +164,45 @@ def paged_attention4(
     """
     if query.ndim != 3:
         raise ValueError("query must be [tokens, q_heads, head_size]")
-    dtype, device = query.dtype, query.device
-    if dtype not in (torch.bfloat16, torch.float16):
+    dtype, device = query.dtype, query.get_device()
+    if dtype not in _HALVES:
         raise NotImplementedError(f"queries must be bfloat16 or float16, not {dtype}")
     tokens, heads, head_size = query.shape
-    codes = cache.codes
-    _, num_blocks, kv_heads, rows, half = codes.shape
+    _, num_blocks, kv_heads, rows, half = cache.codes.shape
     if head_size != 2 * half or heads == 0 or heads % kv_heads:
         raise ValueError(f"query {tuple(query.shape)} does not fit {kv_heads} KV heads of {2 * half}")
     token, head, value = query.stride()
     if value != 1:
         raise ValueError("query heads must be contiguous")
-    if codes.device != device:
+    if cache.codes.get_device() != device:
         raise ValueError("query and cache must live on one device")
     _int32("block_table", block_table, device, 2)
     _int32("seq_lens", seq_lens, device, 1)
     seqs, width = block_table.shape
-    if seq_lens.shape[0] != seqs:
+    if seq_lens.numel() != seqs:
         raise ValueError("block_table must hold one row per sequence")
     start = 0
     if query_start is not None:
         _int32("query_start", query_start, device, 1)
-        if query_start.shape[0] != seqs + 1:
+        if query_start.numel() != seqs + 1:
             raise ValueError("query_start must hold one entry per sequence and one more")
         start = query_start.data_ptr()
     elif tokens != seqs:
         raise ValueError(f"{tokens} query tokens for {seqs} sequences need query_start")
-    if not query.is_cuda:
+    if device < 0:
         _native.require_cuda(query)
     with on_device(device, stream):
         result = _attention_out(query, out)
         if tokens == 0 or seqs == 0:
             return result
-        if workspace is None:
-            workspace = torch.empty(paged_attention4_workspace_bytes(tokens, seqs, heads, kv_heads, head_size),
-                                    dtype=torch.uint8, device=device)
-        elif workspace.dtype != torch.uint8 or workspace.device != device or not workspace.is_contiguous():
-            raise ValueError("workspace must be contiguous uint8 on the query's device")
+        workspace = _scratch(
+            workspace, lambda: paged_attention4_workspace_bytes(tokens, seqs, heads, kv_heads, head_size), query.device)
         out_token, out_head, _ = result.stride()
         _native.call(
             "cb_paged_attention4", query.data_ptr(), 2 * token, 2 * head, tokens, heads, _native.DTYPE_CODES[dtype], start,
             *cache._pages(), num_blocks, rows, kv_heads, head_size, block_table.data_ptr(), block_table.stride(0), width,
             seq_lens.data_ptr(), seqs, float(scale), result.data_ptr(), 2 * out_token, 2 * out_head, workspace.data_ptr(),
-            workspace.numel(), current_handle())
+            workspace.numel(), _raw_stream(device))
         return result
 
 
@@ -233,24 +241,26 @@ def prompt_attention(
     positive.  ``workspace``: ``prompt_attention_workspace_bytes`` of uint8, for callers that keep
     one (two calls that may overlap need two); otherwise allocated per call.
     """
-    if query.ndim != 3 or key.ndim != 3 or value.shape != key.shape:
+    shape, key_shape = query.shape, key.shape
+    if len(shape) != 3 or len(key_shape) != 3 or value.shape != key_shape:
         raise ValueError("query must be [tokens, q_heads, head_size]; key and value [keys, kv_heads, head_size]")
-    if query.dtype not in (torch.bfloat16, torch.float16):
-        raise NotImplementedError(f"prompt attention needs bfloat16 or float16, not {query.dtype}")
-    if not (query.dtype == key.dtype == value.dtype):
+    dtype, device = query.dtype, query.get_device()
+    if dtype not in _HALVES:
+        raise NotImplementedError(f"prompt attention needs bfloat16 or float16, not {dtype}")
+    if key.dtype is not dtype or value.dtype is not dtype:
         raise ValueError("query, key and value must share a dtype")
-    tokens, heads, head_size = query.shape
-    keys, kv_heads, _ = key.shape
-    if key.shape[2] != head_size or kv_heads == 0 or heads == 0 or heads % kv_heads:
-        raise ValueError(f"query {tuple(query.shape)} does not fit keys {tuple(key.shape)}")
-    device = query.device
-    if key.device != device or value.device != device:
+    tokens, heads, head_size = shape
+    keys, kv_heads, key_size = key_shape
+    if key_size != head_size or kv_heads == 0 or heads == 0 or heads % kv_heads:
+        raise ValueError(f"query {tuple(shape)} does not fit keys {tuple(key_shape)}")
+    if key.get_device() != device or value.get_device() != device:
         raise ValueError("query, key and value must live on one device")
-    for name, t in (("query", query), ("key", key), ("value", value)):
-        if t.stride(2) != 1:
-            raise ValueError(f"{name} heads must be contiguous")
+    strides = query.stride(), key.stride(), value.stride()
+    if not (strides[0][2] == strides[1][2] == strides[2][2] == 1):
+        raise ValueError("the heads of query, key and value must be contiguous")
     _int32("query_start", query_start, device, 1)
-    if query_start.shape[0] == 0:
+    seqs = query_start.numel() - 1
+    if seqs < 0:
         raise ValueError("query_start must hold one entry per sequence and one more")
     if key_start is None:
         if keys != tokens:
@@ -258,34 +268,31 @@ def prompt_attention(
         key_start = query_start
     else:
         _int32("key_start", key_start, device, 1)
-        if key_start.shape[0] != query_start.shape[0]:
+        if key_start.numel() != seqs + 1:
             raise ValueError("key_start must hold as many entries as query_start")
     if not scale > 0:
         raise ValueError(f"the scale must be positive, not {scale}")
-    if device_error is not None and (device_error.dtype != torch.int32 or device_error.device != device):
+    if device_error is not None and (device_error.dtype != torch.int32 or device_error.get_device() != device):
         raise ValueError("device_error must be int32 on the query's device")
-    _native.require_cuda(query)
-    seqs = query_start.shape[0] - 1
+    if device < 0:
+        _native.require_cuda(query)
     with on_device(device, stream):
         result = _attention_out(query, out)
         if tokens == 0 or seqs == 0:
             return result
         if keys == 0:
             raise ValueError("prompt attention needs keys")
-        need = prompt_attention_workspace_bytes(tokens, seqs, heads, kv_heads, head_size)
-        if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=device)
-        elif workspace.dtype != torch.uint8 or workspace.device != device or not workspace.is_contiguous():
-            raise ValueError("workspace must be contiguous uint8 on the query's device")
-        strides = []
-        for t in (query, key, value, result):  # (a dimension of one entry may carry any stride)
-            token, head, _ = t.stride()
-            head = head if t.shape[1] > 1 else head_size
-            strides += (2 * (token if t.shape[0] > 1 else head * t.shape[1]), 2 * head)
+        workspace = _scratch(
+            workspace, lambda: prompt_attention_workspace_bytes(tokens, seqs, heads, kv_heads, head_size), query.device)
+        strides = (*strides, result.stride())
+        if tokens == 1 or keys == 1 or heads == 1 or kv_heads == 1:  # dimensions of one may carry any stride
+            strides = [(t if n > 1 else h * (r if h > 1 else head_size), r if h > 1 else head_size)
+                       for (n, h, _), (t, r, _) in zip((shape, key_shape, key_shape, shape), strides)]
+        (q_token, q_head, *_), (k_token, k_head, *_), (v_token, v_head, *_), (out_token, out_head, *_) = strides
         _native.call(
-            "cb_prompt_attention", query.data_ptr(), strides[0], strides[1], key.data_ptr(), strides[2], strides[3],
-            value.data_ptr(), strides[4], strides[5], tokens, keys, heads, kv_heads, head_size,
-            _native.DTYPE_CODES[query.dtype], query_start.data_ptr(), key_start.data_ptr(), seqs, float(scale),
-            result.data_ptr(), strides[6], strides[7], workspace.data_ptr(), workspace.numel(),
-            0 if device_error is None else device_error.data_ptr(), current_handle())
+            "cb_prompt_attention", query.data_ptr(), 2 * q_token, 2 * q_head, key.data_ptr(), 2 * k_token, 2 * k_head,
+            value.data_ptr(), 2 * v_token, 2 * v_head, tokens, keys, heads, kv_heads, head_size,
+            _native.DTYPE_CODES[dtype], query_start.data_ptr(), key_start.data_ptr(), seqs, float(scale),
+            result.data_ptr(), 2 * out_token, 2 * out_head, workspace.data_ptr(), workspace.numel(),
+            0 if device_error is None else device_error.data_ptr(), _raw_stream(device))
         return result
