@@ -1,8 +1,8 @@
 """Attention: of a blend request's staging, of packed prompts, and of decode steps over 4-bit pages.
 
-Blend attention on the tensor cores (cb_blend_attention): the side executor's attention of the computed, possibly pruned, queries over
-the whole staging context: Qwen3BlendExecutor._attention
-(cacheblend_vllm/ascend.py:798-846).  Queries sit at absolute positions and
+Blend attention on the tensor cores (cb_blend_attention): the side executor's
+attention of the computed, possibly pruned, queries over the whole staging
+context: Qwen3BlendExecutor._attention (cacheblend_vllm/ascend.py:798-846).  Queries sit at absolute positions and
 attend every staging row at or before their position; grouped query heads
 share their KV head.  ``prompt_attention`` and ``paged_attention4``: at the end of the file.
 """

@@ -389,11 +389,11 @@ struct Two<__half> {
   }
 };
 
-// Codes of 8 values in four words.  FAR: values may lie beyond
-// fp16's range.  Without them (x - low) / step is at least -1/2, since a 16-bit x in fp16's range
-// is off its fp16 form by 2^-25 at most and a step is 2^-24 at least, so that the nearest whole
-// number (the low bits of v + 1.5 * 2^23) can be cut to 0..15 as an integer, one instruction with
-// the subtraction of the float's upper bits.
+// Codes of 8 values in four words.  FAR: values may lie beyond fp16's range.  Without them
+// (x - low) / step is at least -1/2, since a 16-bit x in fp16's range is off its fp16 form by
+// 2^-25 at most and a step is 2^-24 at least, so that the nearest whole number (the low bits of
+// v + 1.5 * 2^23) can be cut to 0..15 as an integer, one instruction with the subtraction of the
+// float's upper bits.
 template <typename T, bool FAR>
 __device__ __forceinline__ uint32_t codes_of_words(const uint32_t (&w)[4], __half2 pair) {
   const float step = __low2float(pair), base = __high2float(pair);

@@ -18,13 +18,13 @@
 //     subnormal c 2^-24, at bits 4-7 c 2^-20, both exact in the tensor core.  The
 //     factor 2^24 goes into the row's factor, the odd nibbles' 16 into q (K) or
 //     into the output row (V).
-//   * K: the 16 keys of a tile are the M rows, the query rows the N columns
-//     (8: a whole group of query heads usually fits; 16 columns at once, which share
-//     the masked words, ran at half the warps and up to 1.3 times as long), the dimensions of one group
-//     the K steps.  q is scaled per row by a power of two so that its largest
-//     value is in [2^14, 2^15): bf16 and fp16 values are exact in fp16 down to
-//     2^-28 of it.  The low terms are one more product, of the lowest values as they
-//     lie with q's group sums in three fp16 limbs.
+//   * K: the 16 keys of a tile are the M rows, the query rows the N columns, the
+//     dimensions of one group the K steps.  Eight columns: a whole group of query
+//     heads usually fits, and 16 at once, which share the masked words, ran with half
+//     the warps and up to 1.3 times as long.  q is scaled per row by a power of two so
+//     that its largest value is in [2^14, 2^15): bf16 and fp16 values are exact in
+//     fp16 down to 2^-28 of it.  The low terms are one more product, of the lowest
+//     values as they lie with q's group sums in three fp16 limbs.
 //   * V: the dimensions are the M rows, the keys the K steps, P the B operand; a
 //     transposing ldmatrix of 16-bit units (four codes of a key) pairs the same
 //     codes of two keys.  P step'_G is rounded to fp16 (11 bits: 2^-11 relative,
@@ -32,10 +32,11 @@
 //     movmatrix.  The roundings weigh with codes less 8, not with codes: 8 times the
 //     sum of the rounded factors (one more product, of ones) is taken off again and
 //     the low terms are taken at code 8, so that a row's offset does not multiply them
-//     (fp16 outputs of rows around 0: 3.4e-4 off without, 2.1e-4 for one rounding).  M also carries the exponent of the largest step' so that a
-//     factor stays in fp16's range whatever the values' size: at most 2^15, 2^10
-//     when M is set.  M moves only when a factor would pass that, which each lane
-//     sees for itself: the common tile needs no maximum over the warp.
+//     (fp16 outputs of rows around 0: 3.4e-4 off without, 2.4e-4 with, 2.0e-4 for the
+//     rounding of the result alone).  M also carries the exponent of the largest
+//     step' so that a factor stays in fp16's range whatever the values' size: at most
+//     2^15, 2^10 when M is set.  M moves only when a factor would pass that, which each
+//     lane sees for itself: the common tile needs no maximum over the warp.
 // Sums, maxima, steps and the low terms are fp32.
 //
 // Memory: a warp takes tiles of 32 keys of one KV head through a ring of its
@@ -48,9 +49,14 @@
 // its rounds (a tile per warp) and a fixed cost, cut into equal shares, one per
 // CTA, whatever the lengths are; the cut is found on the device from the lengths.
 // Without the fixed cost the CTAs that got many short sequences ran twice as long
-// as the rest (64 sequences of 1 to 8,192 keys: 130 us against 74 then).  The first and last piece of a share may be
-// parts; parts go to the workspace and a second launch joins them in order, so a
-// result does not depend on timing.
+// as the rest (64 sequences of 1 to 8,192 keys: 130 us against 74 then).  The first
+// and last piece of a share may be parts; parts go to the workspace and a second
+// launch joins them in order, so a result does not depend on timing.
+//
+// What bounds it (6 sequences of up to 98,304 keys, 32 query heads on 4: 40 us, 3.8
+// TB/s): about 500 instructions a tile, 160 of them the codes' masks and shifts, at
+// 55 % of the issue slots and 46 % of the ALU pipe with 16 warps an SM, beside some
+// 10 us of launch, first loads and the join.  The memory side alone takes 33 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -63,7 +69,7 @@ constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 8;         // query rows of a piece: the columns of a product
 constexpr int kTileKeys = 32;    // keys of a warp's stage
-constexpr int kStages = 2;       // of a warp's ring; three measured 3 % slower (fewer hits in the L1 beside it)
+constexpr int kStages = 2;       // of a warp's ring; three measured 3 % slower
 constexpr int kCtas = 2 * kSmCount;
 constexpr int kRound = kWarps;   // tiles of a CTA's round: one per warp
 // What a piece costs besides its rounds, in rounds: its first loads, the query operands and

@@ -16,8 +16,9 @@
 // query tiles A and B.  A first launch lists the items of all sequences, the
 // longest first (a counting sort), and the persistent CTAs take them in serpentine
 // order.  Per CTA, 12 warps:
-//   warp 0   Q per item, K tiles through a ring of three (TMA)
-//   warp 3   V tiles through a ring of two, see below
+//   warp 0   Q per item, K tiles through a ring of two (TMA)
+//   warp 3   V tiles through a ring of three, see below (with two, P V waited for V:
+//            it is given back only once the next S is seen)
 //   warp 1   tcgen05.mma: P_A V (t), S_A (t + 1), P_B V (t), S_B (t + 1), ...
 //   warp 2   TMEM: S_A, S_B, O_A, O_B, all 512 columns
 //   warps 4-7 / 8-11   softmax of A / B, a row per thread
