@@ -14,12 +14,14 @@
 // group; a tile is 128 / groups queries (the last rows of a tile whose group
 // count does not divide 128 are idle).  An item is one KV head and a pair of
 // query tiles A and B.  A first launch lists the items of all sequences, the
-// longest first (a counting sort), and the persistent CTAs take them in serpentine
-// order.  Per CTA, 12 warps:
-//   warp 0   Q per item, K tiles through a ring of two (TMA)
+// longest first (a counting sort), and the persistent CTAs take the next one of the
+// list as they come to their last K tiles (dealt out beforehand, the slowest of 148
+// CTAs took 9 % longer than the median).  Per CTA, 12 warps:
+//   warp 0   takes items; Q per item, K tiles through a ring of two (TMA)
 //   warp 3   V tiles through a ring of three, see below (with two, P V waited for V:
 //            it is given back only once the next S is seen)
-//   warp 1   tcgen05.mma: P_A V (t), S_A (t + 1), P_B V (t), S_B (t + 1), ...
+//   warp 1   tcgen05.mma: P_A V (t), S_A (t + 1), P_B V (t), S_B (t + 1), ..., from
+//            an item's last tile straight into the next item's first S
 //   warp 2   TMEM: S_A, S_B, O_A, O_B, all 512 columns
 //   warps 4-7 / 8-11   softmax of A / B, a row per thread
 // P goes back to TMEM over the columns of its own S and is the A operand of P V
@@ -41,6 +43,11 @@
 // epilogue of such an item (rare) adds them to the rows that do see them.
 // Every mbarrier wait is bounded (2 s): a wait that runs out records a code in
 // *device_error, the CTA drains its MMAs and loads, frees TMEM and returns.
+//
+// The softmax warps' code is kept short: what runs once per item is fetched anew each
+// time (about 4 cycles an instruction).  One copy of the tile's code for whole and
+// masked tiles and rolled loops in the epilogue took 9 prompts of 8,500 tokens from
+// 152 to 144 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -57,9 +64,9 @@ constexpr int kVStages = 3;
 constexpr int kThreads = 384;
 constexpr uint32_t kTmemCols = 512;  // S_A [0,128) S_B [128,256) O_A [256,384) O_B [384,512)
 constexpr uint32_t kTmemO = 256;
-// 128 control threads x 40 + 256 softmax threads x 232 = 64512 = 384 x 168 at launch
-constexpr int kRegsControl = 40;
-constexpr int kRegsSoftmax = 232;
+// 128 control threads x 56 + 256 softmax threads x 224 = 64512 = 384 x 168 at launch
+constexpr int kRegsControl = 56;
+constexpr int kRegsSoftmax = 224;
 static_assert(4 * 32 * kRegsControl + 8 * 32 * kRegsSoftmax <= kThreads * 168, "register split");
 constexpr float kRescaleLog2 = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -76,7 +83,7 @@ struct Params {
   int kv_heads, groups, tile_queries;  // queries per tile: 128 / groups
   float scale_log2;                    // scale * log2(e)
   const Item* items;  // null: one sequence, whose items are found from its starts
-  const int* num_items;
+  int* num_items;  // and behind it how many were taken beyond the first of each CTA
   const int32_t* query_start;  // of the one sequence
   const int32_t* key_start;
   int num_queries, num_keys;
@@ -88,16 +95,19 @@ struct Params {
 };
 
 struct Shared {
-  uint64_t q_full, q_empty;
+  uint64_t q_full[kPair], q_empty[kPair];
   uint64_t k_full[kKStages], k_empty[kKStages];
   uint64_t v_landed[kVStages], v_full[kVStages], v_empty[kVStages];
   uint64_t s_full[kPair], p_full[kPair][2];
   uint64_t o_full[kPair], o_empty[kPair];
+  uint64_t work_full, work_empty;
   uint64_t drain;
   uint32_t tmem_base;
   int abort;
   Item one;   // the one sequence: its rows, all its queries, the last key its first query sees
-  int items;  // pairs of query tiles of all sequences
+  int pairs;  // pairs of query tiles of all sequences
+  Item work;  // the CTA's current item, and its KV head; -1: no more
+  int work_head;
   int odd_values;  // a boundary tile held values that are not finite (stays set)
 };
 
@@ -107,19 +117,23 @@ __device__ __forceinline__ void report(const Params& c, Shared& sh, int code) {
 }
 __device__ __forceinline__ bool aborted(Shared& sh) { return *reinterpret_cast<volatile int*>(&sh.abort) != 0; }
 
-// Serpentine: the CTA that got the longest item of a round gets the shortest of the next.
-__device__ __forceinline__ int cta_item(int k) {
-  const int g = static_cast<int>(gridDim.x), c = static_cast<int>(blockIdx.x);
-  return k * g + ((k & 1) ? g - 1 - c : c);
-}
-__device__ __forceinline__ Item load_item(const Params& c, const Shared& sh, int item) {
-  const int pair = item / c.kv_heads;
+__device__ __forceinline__ Item load_item(const Params& c, const Shared& sh, int pair) {
   if (c.items == nullptr) {  // the last queries have the most keys
-    const int first = (sh.items - 1 - pair) * kPair * c.tile_queries;
+    const int first = (sh.pairs - 1 - pair) * kPair * c.tile_queries;
     return Item{sh.one.q_row + first, min(sh.one.queries - first, kPair * c.tile_queries), sh.one.k_row, sh.one.pos + first};
   }
   const int4 v = *reinterpret_cast<const int4*>(c.items + pair);
   return Item{v.x, v.y, v.z, v.w};
+}
+// The k-th item of the CTA, as the thread that loads Q and K publishes it (the first before the
+// CTA's barrier).  False: the wait ran out.
+template <bool WARP>
+__device__ __forceinline__ bool take(Shared& sh, int k, Item& w, int& head) {
+  if (k > 0 && !(WARP ? wait_warp(&sh.work_full, (k - 1) & 1) : wait1(&sh.work_full, (k - 1) & 1))) return false;
+  w = sh.work, head = sh.work_head;
+  if constexpr (WARP) __syncwarp();
+  if (!WARP || (threadIdx.x & 31) == 0) mbar_arrive(&sh.work_empty);
+  return true;
 }
 // A sequence's rows: starts are clamped to the rows there are.
 __device__ __forceinline__ void span(const int32_t* start, int i, int most, int& first, int& length) {
@@ -133,6 +147,16 @@ __device__ __forceinline__ int tile_valid(const Params& c, const Item& w, int x)
 __device__ __forceinline__ int tile_count(const Params& c, const Item& w, int x) {
   const int valid = tile_valid(c, w, x), last = w.pos + x * c.tile_queries + valid - 1;
   return valid > 0 && last >= 0 ? last / kTile + 1 : 0;
+}
+
+// An item for a CTA that will soon be done with its last: the longest that is left.
+__device__ __forceinline__ int claim(const Params& c) {
+  return static_cast<int>(gridDim.x) + (c.items != nullptr ? atomicAdd(c.num_items + 1, 1) : 0);
+}
+__device__ __forceinline__ void publish(const Params& c, Shared& sh, int item) {
+  const int pair = item / c.kv_heads;
+  sh.work_head = pair < sh.pairs ? item - pair * c.kv_heads : -1;
+  if (pair < sh.pairs) sh.work = load_item(c, sh, pair);
 }
 
 template <typename T>
@@ -161,6 +185,31 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]
       "%16};" ::"r"(addr),
       "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
       "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+// 16 rows of 16-byte pieces: lane 4 g + t holds word t of each piece of row g (even registers) and of
+// row g + 8 (odd ones).
+__device__ __forceinline__ void tmem_ld_rows(uint32_t addr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x128b.x8.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15"
+      "}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_rows(uint32_t addr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x128b.x16.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
+      "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31"
+      "}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(addr)
       : "memory");
 }
 template <typename T, int N>
@@ -205,6 +254,21 @@ __device__ __forceinline__ void product_pv(uint32_t tmem_d, uint32_t tmem_p, uin
       "r"(tmem_p), "r"(v_lo), "r"(idesc), "r"(onto ? 1u : 0u), "n"(kDescHi));
 }
 
+// Values that are not finite, to a row that sees them: 32 dimensions of the sum over the item's
+// boundary tiles, where the product had zeros instead.
+template <typename T>
+__device__ __forceinline__ void add_odd(uint32_t (&o)[32], const Params& c, const Item& w, int h, int q, int pos) {
+#pragma unroll 1
+  for (int key = max(w.pos + 1, 0); key <= pos; ++key) {
+    const T* row = reinterpret_cast<const T*>(c.value + (static_cast<int64_t>(w.k_row) + key) * c.value_ts + h * c.value_hs);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const float y = Elem<T>::to_f(row[q * 32 + j]);
+      if (!(fabsf(y) <= 3.4e38f)) o[j] = __float_as_uint(__uint_as_float(o[j]) + y);
+    }
+  }
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
     prompt_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
@@ -221,20 +285,34 @@ __global__ void __launch_bounds__(kThreads, 1)
   unsigned char* v_buf = k_buf + kKStages * kBytes;
 
   if (threadIdx.x == 0) {
-    mbar_init(&sh.q_full, 1);
-    mbar_init(&sh.q_empty, 1);
     for (int s = 0; s < kKStages; ++s) mbar_init(&sh.k_full[s], 1), mbar_init(&sh.k_empty[s], 1);
     for (int s = 0; s < kVStages; ++s)
       mbar_init(&sh.v_landed[s], 1), mbar_init(&sh.v_full[s], 1), mbar_init(&sh.v_empty[s], 1);
     for (int x = 0; x < kPair; ++x) {
+      mbar_init(&sh.q_full[x], 1), mbar_init(&sh.q_empty[x], 1);
       mbar_init(&sh.s_full[x], 1);
       mbar_init(&sh.p_full[x][0], 4), mbar_init(&sh.p_full[x][1], 4);
       mbar_init(&sh.o_full[x], 1), mbar_init(&sh.o_empty[x], 4);
     }
+    mbar_init(&sh.work_full, 1), mbar_init(&sh.work_empty, 10);
     mbar_init(&sh.drain, 1);
     sh.abort = 0;
     sh.odd_values = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the list of items is there
+    if (c.items == nullptr) {
+      int queries, keys;
+      span(c.query_start, 0, c.num_queries, sh.one.q_row, queries);
+      span(c.key_start, 0, c.num_keys, sh.one.k_row, keys);
+      sh.one.queries = queries, sh.one.pos = keys - queries;
+      sh.pairs = (queries + kPair * c.tile_queries - 1) / (kPair * c.tile_queries);
+      publish(c, sh, blockIdx.x);
+    } else {  // (all CTAs' first entries lie in the list's memory, used or not)
+      const int pair = blockIdx.x / c.kv_heads;
+      sh.work = load_item(c, sh, pair);
+      sh.pairs = *c.num_items;
+      sh.work_head = pair < sh.pairs ? blockIdx.x - pair * c.kv_heads : -1;
+    }
   }
   if (warp == 2) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)),
@@ -242,22 +320,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (threadIdx.x == 64) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // the list of items is there
-    if (c.items == nullptr) {
-      int queries, keys;
-      span(c.query_start, 0, c.num_queries, sh.one.q_row, queries);
-      span(c.key_start, 0, c.num_keys, sh.one.k_row, keys);
-      sh.one.queries = queries, sh.one.pos = keys - queries;
-      sh.items = (queries + kPair * c.tile_queries - 1) / (kPair * c.tile_queries);
-    } else {
-      sh.items = *c.num_items;
-    }
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const int items = sh.items * c.kv_heads;
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
@@ -265,39 +330,55 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ------------------------------------------------------ Q and K loads
       if (lane == 0) {
         const uint32_t q_half = static_cast<uint32_t>(c.tile_queries * c.groups * 128);  // bytes of a loaded half tile
-        int t = 0, it = 0;
+        int t = 0, next = 0;
+        int loads[kPair] = {0, 0};           // of Q, per tile of the pair
         uint32_t k_armed = 0, k_parity = 0;  // per stage: a load is in flight / its phase parity
-        int q_armed = -1;
         bool ok = true;
-        for (int k = 0, item = cta_item(0); item < items && ok && !aborted(sh); item = cta_item(++k)) {
-          const Item w = load_item(c, sh, item);
-          const int h = item % c.kv_heads;
-          const int tiles = max(tile_count(c, w, 0), tile_count(c, w, 1));
-          if (tiles == 0) continue;
-          if (!wait1(&sh.q_empty, (it & 1) ^ 1)) { ok = false; break; }
-          const int loaded = tile_valid(c, w, 1) > 0 ? 2 : 1;
-          mbar_expect_tx(&sh.q_full, loaded * kHalves * q_half);
-          for (int x = 0; x < loaded; ++x)
+        for (int k = 0; !aborted(sh); ++k) {
+          if (k > 0) {  // the next item, once every other role has read the last one
+            if (!wait1(&sh.work_empty, (k - 1) & 1)) { ok = false; break; }
+            publish(c, sh, next);
+            mbar_arrive(&sh.work_full);
+          }
+          const Item w = sh.work;
+          const int h = sh.work_head;
+          if (h < 0) break;
+          const int n[kPair] = {tile_count(c, w, 0), tile_count(c, w, 1)};
+          const int tiles = max(n[0], n[1]);
+          if (tiles == 0) {
+            next = claim(c);
+            continue;
+          }
+          auto load_q = [&](int x) -> bool {
+            if (n[x] == 0) return true;
+            if (!wait1(&sh.q_empty[x], (loads[x] & 1) ^ 1)) return false;
+            mbar_expect_tx(&sh.q_full[x], kHalves * q_half);
             for (int i = 0; i < kHalves; ++i)
-              tma_load_4d(q_buf + x * kBytes + i * kHalfBytes, &q_map, &sh.q_full, i * 64, 0, h,
+              tma_load_4d(q_buf + x * kBytes + i * kHalfBytes, &q_map, &sh.q_full[x], i * 64, 0, h,
                           w.q_row + x * c.tile_queries);
-          q_armed = it & 1;
-          ++it;
-          for (int kt = 0; kt < tiles; ++kt, ++t) {
+            ++loads[x];
+            return true;
+          };
+          ok = load_q(0);
+          for (int kt = 0; ok && kt < tiles; ++kt, ++t) {
             const int s = t % kKStages;
+            if (kt == max(tiles - 3, 0)) next = claim(c);  // early enough to hide it, late enough to balance
             if (!wait1(&sh.k_empty[s], ((t / kKStages) & 1) ^ 1)) { ok = false; break; }
             mbar_expect_tx(&sh.k_full[s], kBytes);
             for (int i = 0; i < kHalves; ++i)
               tma_load_3d(k_buf + s * kBytes + i * kHalfBytes, &k_map, &sh.k_full[s], i * 64, h, w.k_row + kt * kTile);
             k_armed |= 1u << s;
             k_parity = (k_parity & ~(1u << s)) | (static_cast<uint32_t>((t / kKStages) & 1) << s);
+            if (kt == 0) ok = load_q(1);  // its tile's slot is the last to be given back
           }
+          if (!ok) break;
         }
         if (!ok) report(c, sh, 1);
         // every armed load has landed before the CTA may exit
         for (int s = 0; s < kKStages; ++s)
           if ((k_armed >> s) & 1u) wait1(&sh.k_full[s], (k_parity >> s) & 1u);
-        if (q_armed >= 0) wait1(&sh.q_full, q_armed);
+        for (int x = 0; x < kPair; ++x)
+          if (loads[x] > 0) wait1(&sh.q_full[x], (loads[x] - 1) & 1);
       }
     } else if (warp == 3) {
       // ------------------------------------------------------ V loads, and a look at boundary tiles
@@ -342,9 +423,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         return true;
       };
       int held = -1, held_from = 0;  // the tile loaded last, where it is not handed on yet
-      for (int k = 0, item = cta_item(0); item < items && ok && !aborted(sh); item = cta_item(++k)) {
-        const Item w = load_item(c, sh, item);
-        const int h = item % c.kv_heads;
+      for (int k = 0; ok && !aborted(sh); ++k) {
+        // the next item may wait for what the products make of the last tile
+        if (k > 0 && held >= 0 && !__all_sync(0xffffffffu, mbar_try(&sh.work_full, (k - 1) & 1))) {
+          ok = hand_on(held, held_from);
+          held = -1;
+        }
+        Item w;
+        int h;
+        if (!ok || !take<true>(sh, k, w, h)) { ok = false; break; }
+        if (h < 0) break;
         const int tiles = max(tile_count(c, w, 0), tile_count(c, w, 1));
         for (int kt = 0; kt < tiles && ok; ++kt, ++t) {
           const int s = t % kVStages;
@@ -377,10 +465,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr uint32_t kDescPV = instr_desc<T, D>() | (1u << 16);  // B (V) MN-major
         const uint32_t q_addr = smem_u32(q_buf), k_addr = smem_u32(k_buf), v_addr = smem_u32(v_buf);
         const uint32_t tmem = sh.tmem_base;
-        int it = 0;                                // items so far
         int ks = 0, vs = 0;                        // ring slots and their parities: running, since the
         uint32_t kp = 0, vp = 0;                   // divisions would stand between two products
-        uint32_t pp[kPair] = {0, 0}, op[kPair] = {1, 1};  // parities of P and of O's release
+        uint32_t pp[kPair] = {0, 0}, op[kPair] = {1, 1}, qp[kPair] = {0, 0};  // parities of P, of O's release, of Q
         bool ok = true;
         auto issue_s = [&](int x) {
 #pragma unroll
@@ -394,38 +481,59 @@ __global__ void __launch_bounds__(kThreads, 1)
           product_pv(tmem + kTmemO + x * kTile, tmem + x * kTile + half * 32, desc_lo_mn(v_rows + half * 64 * 128), kDescPV,
                      onto);
         };
+        auto wait_o = [&](int x) -> bool {  // its last item's rows have been read
+          op[x] ^= 1;
+          return wait1(&sh.o_empty[x], op[x] ^ 1);
+        };
         auto next_k = [&]() {
           if (++ks == kKStages) ks = 0, kp ^= 1;
         };
-        for (int k = 0, item = cta_item(0); item < items && ok && !aborted(sh); item = cta_item(++k)) {
-          const Item w = load_item(c, sh, item);
-          const int n[kPair] = {tile_count(c, w, 0), tile_count(c, w, 1)};
-          const int tiles = max(n[0], n[1]);
-          if (tiles == 0) continue;
-          if (!wait1(&sh.q_full, it & 1) || !wait1(&sh.k_full[ks], kp)) { ok = false; break; }
-          ++it;
-          tc_fence_after();
-#pragma unroll
-          for (int x = 0; x < kPair; ++x)
-            if (n[x] > 0) issue_s(x);
-          next_k();
-          ok = wait1(&sh.v_full[vs], vp);  // (V of each next tile is looked for behind P V)
-#pragma unroll
-          for (int x = 0; x < kPair; ++x)
-            if (n[x] > 0) ok = wait1(&sh.o_empty[x], op[x]) && ok, op[x] ^= 1;
+        int n[kPair], items = 0;
+        // the next item; false: none.  Its key tiles are 0 where its queries see nothing.
+        auto next_item = [&]() -> bool {
+          Item w;
+          int h;
+          if (!take<false>(sh, items++, w, h)) ok = false;
+          if (!ok || h < 0) return false;
+          n[0] = tile_count(c, w, 0), n[1] = tile_count(c, w, 1);
+          return true;
+        };
+        // the first S of query tile x of that item
+        auto start = [&](int x) {
+          if (n[x] > 0 && ok) {
+            ok = wait1(&sh.q_full[x], qp[x]) && wait1(&sh.k_full[ks], kp);
+            qp[x] ^= 1;
+            tc_fence_after();
+            if (ok) issue_s(x);
+          }
+          if (x == 1) next_k();
+        };
+        bool more = next_item(), started = false;
+        while (more && ok && !aborted(sh)) {
+          const int m[kPair] = {n[0], n[1]};
+          const int tiles = max(m[0], m[1]);
+          if (tiles == 0) {
+            more = next_item();
+            continue;
+          }
+          if (!started) start(0), start(1);
+          started = false;
+          ok = ok && wait1(&sh.v_full[vs], vp);  // (V of each next tile is looked for behind P V)
           int kt = 0;
           // Tiles that both query tiles have a successor of.  Every look at a barrier stands where the
           // products issued before it still have time to run (the issue of a product waits for the
           // third before it, so 200 cycles); a wait that ran out is acted on at the end of the round.
-          for (; ok && kt + 1 < min(n[0], n[1]); ++kt) {
+          for (; ok && kt + 1 < min(m[0], m[1]); ++kt) {
             const uint32_t v_rows = v_addr + vs * kBytes;
             const bool onto = kt > 0;
-            ok = wait1(&sh.p_full[0][0], pp[0]);
+            if (!onto) ok = wait_o(0);
+            ok = wait1(&sh.p_full[0][0], pp[0]) && ok;
             issue_pv(0, 0, v_rows, onto);
             ok = wait1(&sh.k_full[ks], kp) && ok;
             ok = wait1(&sh.p_full[0][1], pp[0]) && ok;
             issue_pv(0, 1, v_rows, true);
             issue_s(0);
+            if (!onto) ok = wait_o(1) && ok;
             ok = wait1(&sh.p_full[1][0], pp[1]) && ok;
             issue_pv(1, 0, v_rows, onto);
             ok = wait1(&sh.p_full[1][1], pp[1]) && ok;
@@ -436,27 +544,34 @@ __global__ void __launch_bounds__(kThreads, 1)
             next_k();
             pp[0] ^= 1, pp[1] ^= 1;
           }
-          // the last tiles of either
+          // the last tiles of either; behind the very last ones the next item's first S
           for (; ok && kt < tiles; ++kt) {
             const uint32_t v_rows = v_addr + vs * kBytes;
-            bool have_k = kt + 1 >= tiles;
+            const bool final = kt + 1 == tiles;
+            bool have_k = final;
 #pragma unroll
             for (int x = 0; x < kPair; ++x) {
-              if (kt >= n[x]) continue;
-              ok = wait1(&sh.p_full[x][0], pp[x]) && ok;
-              issue_pv(x, 0, v_rows, kt > 0);
-              if (!have_k) ok = wait1(&sh.k_full[ks], kp) && ok;
-              have_k = true;
-              ok = wait1(&sh.p_full[x][1], pp[x]) && ok;
-              issue_pv(x, 1, v_rows, true);
-              pp[x] ^= 1;
-              if (kt + 1 < n[x])
-                issue_s(x);
-              else
-                umma_commit(&sh.o_full[x]);
+              if (kt < m[x]) {
+                if (kt == 0) ok = wait_o(x) && ok;
+                ok = wait1(&sh.p_full[x][0], pp[x]) && ok;
+                issue_pv(x, 0, v_rows, kt > 0);
+                if (!have_k) ok = wait1(&sh.k_full[ks], kp) && ok;
+                have_k = true;
+                ok = wait1(&sh.p_full[x][1], pp[x]) && ok;
+                issue_pv(x, 1, v_rows, true);
+                pp[x] ^= 1;
+                if (kt + 1 < m[x])
+                  issue_s(x);
+                else
+                  umma_commit(&sh.o_full[x]);
+              }
+              if (final) {
+                if (x == 0) more = next_item(), started = more && max(n[0], n[1]) > 0;
+                if (started) start(x);
+              }
             }
             if (++vs == kVStages) vs = 0, vp ^= 1;
-            if (kt + 1 < tiles) {
+            if (!final) {
               next_k();
               ok = ok && wait1(&sh.v_full[vs], vp);
             }
@@ -477,6 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_tmem = sh.tmem_base + x * kTile + lane_off;
     const uint32_t o_tmem = sh.tmem_base + kTmemO + x * kTile + lane_off;
     const int query_in_tile = row_in_tile / c.groups, group = row_in_tile - query_in_tile * c.groups;
+    const int first_query = x * c.tile_queries + ew * 32 / c.groups;  // of the warp's rows
     // This warpgroup gives back what its products were the last to read: K of a tile (and Q with the
     // item's last) once its S is there, V once the next S, or O, is.  The MMA thread would need a
     // commit for each, and a commit behind a commit holds it up until the first has arrived (470
@@ -484,34 +600,41 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool keeper = ew == 0 && lane == 0;
     int t = 0, o_count = 0, tiles_before = 0;
     bool ok = true;
-    for (int k = 0, item = cta_item(0); item < items && ok; item = cta_item(++k)) {
-      const Item w = load_item(c, sh, item);
-      const int h = item % c.kv_heads;
+    for (int k = 0;; ++k) {
+      Item w;
+      int h;
+      if (!take<true>(sh, k, w, h)) { ok = false; break; }
+      if (h < 0) break;
       const int n = tile_count(c, w, x), n_b = tile_count(c, w, 1);
       auto last_reader = [&](int kt) { return x == 1 || kt >= n_b; };
       const bool store = query_in_tile < tile_valid(c, w, x);
       const int pos = w.pos + x * c.tile_queries + query_in_tile;  // the last key this row sees
       float m_used = -INFINITY;  // log2-domain maximum the exponentials are taken against
       float l = 0.0f;
-      // A tile of S; MASKED: some row of this warp does not see all of it.  Two copies, so that the
-      // loop that runs longest is short: with the masks' code in it, skipped, it ran 6 % slower.
-      auto softmax_tile = [&](auto masked_tag, int kt) {
-        constexpr bool MASKED = decltype(masked_tag)::value;
+      // whole tiles: up to the last key that the warp's first row sees
+      const int first_pos = w.pos + first_query;
+      const int whole = min(max(first_pos + 1, 0) / kTile, n);
+      // a tile of S
+      auto softmax_tile = [&](int kt) {
         if (keeper) {
           if (last_reader(kt)) mbar_arrive(&sh.k_empty[(tiles_before + kt) % kKStages]);
           if (kt > 0 && last_reader(kt - 1)) mbar_arrive(&sh.v_empty[(tiles_before + kt - 1) % kVStages]);
-          if (kt + 1 == n && last_reader(kt)) mbar_arrive(&sh.q_empty);
+          if (kt + 1 == n) mbar_arrive(&sh.q_empty[x]);
         }
         tc_fence_after();
         uint32_t v[4][32];
 #pragma unroll
         for (int q = 0; q < 4; ++q) tmem_ld32(s_tmem + q * 32, v[q]);
         tmem_wait_ld();
-        if constexpr (MASKED) {
-          const int valid = min(max(pos - kt * kTile + 1, 0), kTile);
+        if (kt >= whole) {
+          const int valid = pos - kt * kTile + 1;
 #pragma unroll
-          for (int j = 0; j < kTile; ++j)
-            if (j >= valid) v[j >> 5][j & 31] = __float_as_uint(-INFINITY);
+          for (int q = 0; q < 4; ++q)  // most of a diagonal tile's quarters are seen by the whole warp
+            if (!__all_sync(0xffffffffu, valid >= (q + 1) * 32)) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (q * 32 + j >= valid) v[q][j] = __float_as_uint(-INFINITY);
+            }
         }
         auto s_of = [&](int j) { return __uint_as_float(v[j >> 5][j & 31]); };
         float mx[4];
@@ -567,23 +690,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float2 st = __fadd2_rn(__fadd2_rn(sm[0], sm[1]), __fadd2_rn(sm[2], sm[3]));
         l += st.x + st.y;
       };
-      // whole tiles: up to the last key that the warp's first row sees
-      const int first_pos = w.pos + x * c.tile_queries + ew * 32 / c.groups;
-      const int whole = min(max(first_pos + 1, 0) / kTile, n);
       int kt = 0;
 #pragma unroll 1
-      for (; kt < whole; ++kt, ++t) {
+      for (; kt < n; ++kt, ++t) {
         if (!wait_warp(&sh.s_full[x], t & 1)) { ok = false; break; }
-        softmax_tile(std::false_type{}, kt);
-      }
-#pragma unroll 1
-      for (; ok && kt < n; ++kt, ++t) {
-        if (!wait_warp(&sh.s_full[x], t & 1)) { ok = false; break; }
-        softmax_tile(std::true_type{}, kt);
+        softmax_tile(kt);
       }
       if (!ok) break;
-      T* dst = reinterpret_cast<T*>(c.out + (static_cast<int64_t>(w.q_row) + x * c.tile_queries + query_in_tile) * c.out_ts +
-                                    static_cast<int64_t>(h * c.groups + group) * c.out_hs);
       if (n > 0) {
         if (!wait_warp(&sh.o_full[x], o_count & 1)) { ok = false; break; }
         ++o_count;
@@ -594,38 +707,59 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the P V of the item's boundary tiles came after their look-through
       const bool odd = *reinterpret_cast<volatile int*>(&sh.odd_values) != 0;
       const bool seen = n > 0 && pos >= 0;
-      const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+      const float inv = l != 0.0f ? __fdividef(1.0f, l) : 0.0f;  // (2 ulp at most)
+      // A row per thread, so a store of 16 bytes each would touch 32 lines (47 cycles of the load/store
+      // unit, 6,000 for the item's two tiles, with the other warps' loads behind them).  The packed
+      // rows go back to TMEM, over O, and come again as (row, 16 bytes) by lane / 4 and lane % 4:
+      // 64 bytes of eight rows a store.
+      char* const dst = c.out + (static_cast<int64_t>(w.q_row) + x * c.tile_queries + query_in_tile) * c.out_ts +
+                        static_cast<int64_t>(h * c.groups + group) * c.out_hs;
+      auto row_of = [&](int i) {  // where the lane's piece of its i-th row goes
+        const unsigned long long at =
+            __shfl_sync(0xffffffffu, store ? reinterpret_cast<unsigned long long>(dst) : 0ull, i * 8 + (lane >> 2));
+        return at == 0 ? nullptr : reinterpret_cast<char*>(at) + (lane & 3) * 16;
+      };
+      if (n > 0) {
 #pragma unroll 1
-      for (int q = 0; q < D / 32; ++q) {
-        uint32_t o[32];
-        if (n > 0) {
+        for (int q = 0; q < D / 32; ++q) {
+          uint32_t o[32];
           tmem_ld32(o_tmem + q * 32, o);
           tmem_wait_ld();
-        }
-        if (!store) continue;
-        if (odd && seen) {  // values that are not finite: to the rows that see them
-          for (int key = max(w.pos + 1, 0); key <= pos; ++key) {
-            const T* row = reinterpret_cast<const T*>(c.value + (static_cast<int64_t>(w.k_row) + key) * c.value_ts + h * c.value_hs);
+          if (odd && seen && store) add_odd<T>(o, c, w, h, q, pos);
+          uint32_t word[16];  // word 4 t + i of the 64 bytes at column 4 i + t
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float y = Elem<T>::to_f(row[q * 32 + j]);
-              if (!(fabsf(y) <= 3.4e38f)) o[j] = __float_as_uint(__uint_as_float(o[j]) + y);
-            }
+          for (int j = 0; j < 16; ++j) {
+            const float2 y = __fmul2_rn(make_float2(__uint_as_float(o[2 * j]), __uint_as_float(o[2 * j + 1])), make_float2(inv, inv));
+            word[(j & 3) * 4 + (j >> 2)] = pack2<T>(y.x, y.y);
+          }
+          tmem_st16(o_tmem + q * 16, word);
+        }
+        tmem_wait_st();
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {  // 16 rows
+          uint32_t v[D / 4];
+          tmem_ld_rows(o_tmem + (static_cast<uint32_t>(half * 16) << 16), v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            char* const row = row_of(half * 2 + i);
+            if (row != nullptr)
+#pragma unroll
+              for (int q = 0; q < D / 32; ++q)
+                *reinterpret_cast<uint4*>(row + q * 64) =
+                    make_uint4(v[q * 8 + i], v[q * 8 + 2 + i], v[q * 8 + 4 + i], v[q * 8 + 6 + i]);
           }
         }
-#pragma unroll
-        for (int j = 0; j < 32; j += 8) {
-          uint32_t p[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            p[i] = seen ? pack2<T>(__uint_as_float(o[j + 2 * i]) * inv, __uint_as_float(o[j + 2 * i + 1]) * inv) : 0u;
-          *reinterpret_cast<uint4*>(dst + q * 32 + j) = make_uint4(p[0], p[1], p[2], p[3]);
-        }
-      }
-      if (n > 0) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.o_empty[x]);
+      } else {  // the item's rows see nothing
+        for (int i = 0; i < 4; ++i) {
+          char* const row = row_of(i);
+          if (row != nullptr)
+#pragma unroll
+            for (int q = 0; q < D / 32; ++q) *reinterpret_cast<uint4*>(row + q * 64) = make_uint4(0, 0, 0, 0);
+        }
       }
     }
     if (!ok && lane == 0) report(c, sh, 3);
@@ -696,7 +830,7 @@ __global__ void __launch_bounds__(kListThreads) list_kernel(const int32_t* __res
       }
       before += base - sum;
       for (int j = 0; j < kPer; ++j) count[threadIdx.x * kPer + j] = before, before += mine[j];
-      if (threadIdx.x == 0) *num_items = min(total, capacity);
+      if (threadIdx.x == 0) num_items[0] = min(total, capacity), num_items[1] = 0;
       __syncthreads();
     }
   }
@@ -830,8 +964,8 @@ extern "C" int cb_prompt_attention(const void* query, int64_t query_token_stride
   c.query_start = query_start, c.key_start = key_start;
   c.num_queries = static_cast<int>(num_queries), c.num_keys = static_cast<int>(num_keys);
   // One sequence's items are an arithmetic series: no list, and one launch less (a 301-token prompt:
-  // 14.4 us with it).
-  if (num_seqs > 1) {
+  // 14.4 us with it).  Not where CTAs take several: the list kernel also clears their counter.
+  if (num_seqs > 1 || items * num_kv_heads > kSmCount) {
     int* num_items = static_cast<int*>(workspace);
     prompt::Item* list = reinterpret_cast<prompt::Item*>(static_cast<char*>(workspace) + 256);
     c.items = list, c.num_items = num_items;

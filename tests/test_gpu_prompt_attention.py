@@ -128,6 +128,26 @@ def test_more_queries_than_keys(cuda):
     _check(got, q, k, v, [0, 40, 90], [0, 0, 50], 0.125)
 
 
+@pytest.mark.parametrize("lengths,keys", [
+    ([2500], [2500]),  # one sequence, several items per CTA
+    ([70, 1, 400, 33, 64, 900, 16] * 6, [0, 1, 300, 0, 20, 1200, 500] * 6),  # many that see nothing, among others
+    ([40] * 90, [0] * 89 + [7]),  # almost only those
+    ([17] * 200, [17] * 200),  # one tile each: the next item follows at once
+])
+def test_several_items_per_cta(cuda, lengths, keys):
+    q, k, v = _inputs(cuda, sum(lengths), sum(keys), 16, 8, 64 if len(lengths) > 100 else 128, torch.bfloat16, 11)
+    starts, key_starts = _starts(lengths, cuda), _starts(keys, cuda)
+    workspace = torch.full((prompt_attention_workspace_bytes(len(q), len(lengths), 16, 8, q.shape[2]),), 255, dtype=torch.uint8,
+                           device=cuda)
+    error = torch.zeros(1, dtype=torch.int32, device=cuda)
+    got = prompt_attention(q, k, v, starts, 0.1, key_start=key_starts, workspace=workspace, device_error=error)
+    for _ in range(3):  # the workspace as the call before left it
+        again = prompt_attention(q, k, v, starts, 0.1, key_start=key_starts, workspace=workspace, device_error=error)
+        assert bool((got.view(torch.int16) == again.view(torch.int16)).all())
+    assert int(error) == 0
+    _check(got, q, k, v, starts.tolist(), key_starts.tolist(), 0.1)
+
+
 def test_strides_and_rows_behind(cuda):
     """Slices of one projection's output; rows of no sequence stay as they were."""
     heads, kv_heads, head, tokens = 8, 2, 128, 333
