@@ -15,7 +15,7 @@
 // count does not divide 128 are idle).  An item is one KV head and a pair of
 // query tiles A and B.  A first launch lists the items of all sequences, the
 // longest first (a counting sort), and the persistent CTAs take the next one of the
-// list as they come to their last K tiles (dealt out beforehand, the slowest of 148
+// list as they come to their last two K tiles (dealt out beforehand, the slowest of 148
 // CTAs took 9 % longer than the median).  Per CTA, 12 warps:
 //   warp 0   takes items; Q per item, K tiles through a ring of two (TMA)
 //   warp 3   V tiles through a ring of three, see below (with two, P V waited for V:
@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = load_q(0);
           for (int kt = 0; ok && kt < tiles; ++kt, ++t) {
             const int s = t % kKStages;
-            if (kt == max(tiles - 3, 0)) next = claim(c);  // early enough to hide it, late enough to balance
+            if (kt == max(tiles - 2, 0)) next = claim(c);  // its latency is hidden, and no CTA holds two for long
             if (!wait1(&sh.k_empty[s], ((t / kKStages) & 1) ^ 1)) { ok = false; break; }
             mbar_expect_tx(&sh.k_full[s], kBytes);
             for (int i = 0; i < kHalves; ++i)
