@@ -559,6 +559,20 @@ CB_API int cb_prompt_attention(const void* query, int64_t query_token_stride,
                                int64_t out_head_stride, void* workspace, int64_t workspace_bytes,
                                int32_t* device_error, void* stream);
 
+/*
+ * One of the five calls above (cb_append_paged_kv, cb_append_paged_kv4, cb_gather_paged_kv4,
+ * cb_paged_attention4, cb_prompt_attention) with its arguments in order as 64-bit words:
+ * pointers and integers by value, a float as the bits of a double.  For bindings whose
+ * argument conversion costs more than the launch.  device: the one that holds the memory
+ * (it saves the look-up that the others make where the stream is NULL).
+ */
+#define CB_PACKED_APPEND_PAGED_KV 0
+#define CB_PACKED_APPEND_PAGED_KV4 1
+#define CB_PACKED_GATHER_PAGED_KV4 2
+#define CB_PACKED_PAGED_ATTENTION4 3
+#define CB_PACKED_PROMPT_ATTENTION 4
+CB_API int cb_call_packed(int entry, int device, const int64_t* words, int64_t num_words);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -164,6 +165,15 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32,
          _ptr, _ptr, _i64, ctypes.c_float, _ptr, _i64, _i64, _ptr, _i64, _ptr, _ptr],
     ),
+    "cb_call_packed": (_i32, [_i32, _i32, ctypes.c_char_p, _i64]),
+}
+
+# name -> (entry code, packer of its arguments into 64-bit words, their number)
+PACKED = {
+    name: (code, struct.Struct("=" + "".join("d" if a is ctypes.c_float else "q" for a in SIGNATURES[name][1])).pack,
+           len(SIGNATURES[name][1]))
+    for code, name in enumerate(("cb_append_paged_kv", "cb_append_paged_kv4", "cb_gather_paged_kv4", "cb_paged_attention4",
+                                 "cb_prompt_attention"))
 }
 
 _lock = threading.Lock()
@@ -197,15 +207,27 @@ def load_library() -> ctypes.CDLL:
 
 def call(name: str, *args) -> None:
     """Invoke a C-ABI entry point and translate its status into an exception."""
-    lib = load_library()
-    rc = getattr(lib, name)(*args)
+    rc = getattr(load_library(), name)(*args)
     if rc != CB_OK:
-        message = lib.cb_last_error().decode(errors="replace")
-        if rc == CB_ERR_INVALID:
-            raise ValueError(f"{name}: {message}")
-        if rc == CB_ERR_UNSUPPORTED:
-            raise NotImplementedError(f"{name}: {message}")
-        raise RuntimeError(f"{name}: {message}")
+        _raise(name, rc)
+
+
+def call_packed(name: str, device: int, *args) -> None:
+    """``call`` of an entry in PACKED for tensors on ``device``, its arguments converted in one go
+    (33 of them: 1 us, not 3)."""
+    entry, pack, words = PACKED[name]
+    rc = (_lib or load_library()).cb_call_packed(entry, device, pack(*args), words)
+    if rc != CB_OK:
+        _raise(name, rc)
+
+
+def _raise(name: str, rc: int) -> None:
+    message = load_library().cb_last_error().decode(errors="replace")
+    if rc == CB_ERR_INVALID:
+        raise ValueError(f"{name}: {message}")
+    if rc == CB_ERR_UNSUPPORTED:
+        raise NotImplementedError(f"{name}: {message}")
+    raise RuntimeError(f"{name}: {message}")
 
 
 def require_cuda(*tensors: torch.Tensor) -> None:

@@ -212,11 +212,12 @@ def _append(entry: str, rotary_emb, positions, key, value, query, rows: tuple, s
             q_heads, q, out = query.shape[1], query.data_ptr(), turned.data_ptr()
         if tokens == 0:
             return turned
-        _native.call(entry, key.data_ptr(), of_key[0] * size, of_key[1] * size, value.data_ptr(), of_value[0] * size,
-                     of_value[1] * size, q, of_query[0] * size, of_query[1] * size, out, q_heads * head_size * size,
-                     head_size * size, tokens, q_heads, heads, head_size, _native.DTYPE_CODES[dtype], where,
-                     0 if table is None else table.data_ptr(), table_code, max_position, rotary_dim, neox, *pages,
-                     num_blocks, block_size, slots.data_ptr(), _raw_stream(device))
+        _native.call_packed(
+            entry, device, key.data_ptr(), of_key[0] * size, of_key[1] * size, value.data_ptr(), of_value[0] * size,
+            of_value[1] * size, q, of_query[0] * size, of_query[1] * size, out, q_heads * head_size * size,
+            head_size * size, tokens, q_heads, heads, head_size, _native.DTYPE_CODES[dtype], where,
+            0 if table is None else table.data_ptr(), table_code, max_position, rotary_dim, neox, *pages, num_blocks,
+            block_size, slots.data_ptr(), _raw_stream(device))
         return turned
 
 
@@ -330,7 +331,7 @@ def gather_paged_kv4(
             return result
         size = result.element_size()
         plane, token, head, _ = result.stride()
-        _native.call("cb_gather_paged_kv4", *cache._pages(), num_blocks, rows, heads, 2 * half, slots.data_ptr(), tokens,
-                     result.data_ptr(), plane * size, token * size, head * size, _native.DTYPE_CODES[dtype],
-                     _raw_stream(device))
+        _native.call_packed(
+            "cb_gather_paged_kv4", device, *cache._pages(), num_blocks, rows, heads, 2 * half, slots.data_ptr(), tokens,
+            result.data_ptr(), plane * size, token * size, head * size, _native.DTYPE_CODES[dtype], _raw_stream(device))
         return result

@@ -10,6 +10,7 @@ share their KV head.  ``prompt_attention`` and ``paged_attention4``: at the end 
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -137,6 +138,9 @@ def paged_attention4_workspace_bytes(num_tokens: int, num_seqs: int, num_q_heads
     return int(size.value)
 
 
+_decode_bytes = functools.lru_cache(paged_attention4_workspace_bytes)  # a size depends on sizes alone
+
+
 def paged_attention4(
     query: torch.Tensor,
     cache: PagedKV4,
@@ -196,11 +200,11 @@ def paged_attention4(
         if tokens == 0 or seqs == 0:
             return result
         workspace = _scratch(
-            workspace, lambda: paged_attention4_workspace_bytes(tokens, seqs, heads, kv_heads, head_size), query.device)
+            workspace, lambda: _decode_bytes(tokens, seqs, heads, kv_heads, head_size), query.device)
         out_token, out_head, _ = result.stride()
-        _native.call(
-            "cb_paged_attention4", query.data_ptr(), 2 * token, 2 * head, tokens, heads, _native.DTYPE_CODES[dtype], start,
-            *cache._pages(), num_blocks, rows, kv_heads, head_size, block_table.data_ptr(), block_table.stride(0), width,
+        _native.call_packed(
+            "cb_paged_attention4", device, query.data_ptr(), 2 * token, 2 * head, tokens, heads,
+            _native.DTYPE_CODES[dtype], start, *cache._pages(), num_blocks, rows, kv_heads, head_size, block_table.data_ptr(), block_table.stride(0), width,
             seq_lens.data_ptr(), seqs, float(scale), result.data_ptr(), 2 * out_token, 2 * out_head, workspace.data_ptr(),
             workspace.numel(), _raw_stream(device))
         return result
@@ -212,6 +216,9 @@ def prompt_attention_workspace_bytes(num_queries: int, num_seqs: int, num_q_head
     _native.call("cb_prompt_attention_workspace_size", num_queries, num_seqs, num_q_heads, num_kv_heads, head_size,
                  ctypes.addressof(size))
     return int(size.value)
+
+
+_prompt_bytes = functools.lru_cache(prompt_attention_workspace_bytes)
 
 
 def prompt_attention(
@@ -283,15 +290,15 @@ def prompt_attention(
         if keys == 0:
             raise ValueError("prompt attention needs keys")
         workspace = _scratch(
-            workspace, lambda: prompt_attention_workspace_bytes(tokens, seqs, heads, kv_heads, head_size), query.device)
+            workspace, lambda: _prompt_bytes(tokens, seqs, heads, kv_heads, head_size), query.device)
         strides = (*strides, result.stride())
         if tokens == 1 or keys == 1 or heads == 1 or kv_heads == 1:  # dimensions of one may carry any stride
             strides = [(t if n > 1 else h * (r if h > 1 else head_size), r if h > 1 else head_size)
                        for (n, h, _), (t, r, _) in zip((shape, key_shape, key_shape, shape), strides)]
         (q_token, q_head, *_), (k_token, k_head, *_), (v_token, v_head, *_), (out_token, out_head, *_) = strides
-        _native.call(
-            "cb_prompt_attention", query.data_ptr(), 2 * q_token, 2 * q_head, key.data_ptr(), 2 * k_token, 2 * k_head,
-            value.data_ptr(), 2 * v_token, 2 * v_head, tokens, keys, heads, kv_heads, head_size,
+        _native.call_packed(
+            "cb_prompt_attention", device, query.data_ptr(), 2 * q_token, 2 * q_head, key.data_ptr(), 2 * k_token,
+            2 * k_head, value.data_ptr(), 2 * v_token, 2 * v_head, tokens, keys, heads, kv_heads, head_size,
             _native.DTYPE_CODES[dtype], query_start.data_ptr(), key_start.data_ptr(), seqs, float(scale),
             result.data_ptr(), 2 * out_token, 2 * out_head, workspace.data_ptr(), workspace.numel(),
             0 if device_error is None else device_error.data_ptr(), _raw_stream(device))

@@ -21,6 +21,13 @@ void clear_error();
 // instance considers current.
 int bind_stream(void* stream, const void* device_ptr);
 
+// While one lives, bind_stream on its thread takes `device` for the legacy NULL stream and does
+// not look at the pointer.
+struct NullStreamDevice {
+  explicit NullStreamDevice(int device);
+  ~NullStreamDevice();
+};
+
 // Converts the launch status into CB_OK / CB_ERR_CUDA.
 int launch_status(const char* kernel);
 

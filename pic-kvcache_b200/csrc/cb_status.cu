@@ -14,6 +14,7 @@ namespace cb {
 
 namespace {
 thread_local char g_last_error[512] = {0};
+thread_local int g_null_stream_device = -1;
 }
 
 void set_error(const char* fmt, ...) {
@@ -24,6 +25,9 @@ void set_error(const char* fmt, ...) {
 }
 
 void clear_error() { g_last_error[0] = 0; }
+
+NullStreamDevice::NullStreamDevice(int device) { g_null_stream_device = device; }
+NullStreamDevice::~NullStreamDevice() { g_null_stream_device = -1; }
 
 int bind_stream(void* stream, const void* device_ptr) {
   clear_error();
@@ -44,6 +48,8 @@ int bind_stream(void* stream, const void* device_ptr) {
       set_error("cudaStreamGetDevice failed: %s", cudaGetErrorString(e));
       return CB_ERR_CUDA;
     }
+  } else if (g_null_stream_device >= 0) {
+    want = g_null_stream_device;
   } else if (device_ptr != nullptr) {
     // Legacy default stream: the output tensor's device decides.
     cudaPointerAttributes attr;

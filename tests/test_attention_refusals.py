@@ -98,3 +98,27 @@ def test_c_entries_refuse_before_any_device_work():
     assert prompt(dtype=2) == _native.CB_ERR_UNSUPPORTED
     assert prompt(head=32) == _native.CB_ERR_UNSUPPORTED
     assert prompt(keys=-1) == _native.CB_ERR_INVALID
+
+
+def test_packed_calls_refuse_alike():
+    """cb_call_packed: the entries' own refusals, and those of words that fit no entry."""
+    lib = _native.load_library()
+    assert [code for code, _, _ in _native.PACKED.values()] == list(range(5))
+    for name, (code, pack, count) in _native.PACKED.items():
+        words = pack(*[0] * count)
+        assert len(words) == 8 * count
+        direct = getattr(lib, name)(*[0] * count)
+        message = lib.cb_last_error()
+        packed = lib.cb_call_packed(code, 0, words, count)
+        if packed != _native.CB_ERR_CUDA:  # (no device here: it cannot be made current)
+            assert packed == direct and lib.cb_last_error() == message
+        assert lib.cb_call_packed(code, 0, words, count - 1) == _native.CB_ERR_INVALID
+        assert b"words" in lib.cb_last_error()
+        assert lib.cb_call_packed(code, -1, words, count) == _native.CB_ERR_INVALID
+        assert lib.cb_call_packed(code, 0, None, count) == _native.CB_ERR_INVALID
+    assert lib.cb_call_packed(5, 0, b"\0" * 64, 8) == _native.CB_ERR_INVALID
+    code, pack, count = _native.PACKED["cb_prompt_attention"]
+    values = [0] * count
+    values[14] = 1 << 32  # the element type's code is an int
+    assert lib.cb_call_packed(code, 0, pack(*values), count) == _native.CB_ERR_INVALID
+    assert b"fit" in lib.cb_last_error()
