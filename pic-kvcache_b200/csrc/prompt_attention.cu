@@ -13,8 +13,8 @@
 // Rows are (query, group) pairs of one KV head, so a K / V tile serves the whole
 // group; a tile is 128 / groups queries (the last rows of a tile whose group
 // count does not divide 128 are idle).  An item is one KV head and a pair of
-// query tiles A and B.  A first launch lists the items of all sequences, the
-// longest first (a counting sort), and the persistent CTAs take the next one of the
+// query tiles A and B.  Where there are more of them than SMs, a first launch lists
+// the items of all sequences, the longest first (a counting sort), and the persistent CTAs take the next one of the
 // list as they come to their last two K tiles (dealt out beforehand, the slowest of 148
 // CTAs took 9 % longer than the median).  Per CTA, 12 warps:
 //   warp 0   takes items; Q per item, K tiles through a ring of two (TMA)
@@ -85,11 +85,11 @@ struct alignas(16) Item {
 struct Params {
   int kv_heads, groups, tile_queries;  // queries per tile: 128 / groups
   float scale_log2;                    // scale * log2(e)
-  const Item* items;  // null: one sequence, whose items are found from its starts
+  const Item* items;  // null: an item per CTA, found from the sequences' starts
   int* num_items;  // and behind it how many were taken beyond the first of each CTA
-  const int32_t* query_start;  // of the one sequence
+  const int32_t* query_start;  // without a list
   const int32_t* key_start;
-  int num_queries, num_keys;
+  int num_seqs, num_queries, num_keys;
   const char* value;  // for the epilogue of items with values that are not finite
   int64_t value_ts, value_hs;
   char* out;
@@ -107,7 +107,6 @@ struct Shared {
   uint64_t drain;
   uint32_t tmem_base;
   int abort;
-  Item one;   // the one sequence: its rows, all its queries, the last key its first query sees
   int pairs;  // pairs of query tiles of all sequences
   Item work;  // the CTA's current item, and its KV head; -1: no more
   int work_head;
@@ -120,11 +119,7 @@ __device__ __forceinline__ void report(const Params& c, Shared& sh, int code) {
 }
 __device__ __forceinline__ bool aborted(Shared& sh) { return *reinterpret_cast<volatile int*>(&sh.abort) != 0; }
 
-__device__ __forceinline__ Item load_item(const Params& c, const Shared& sh, int pair) {
-  if (c.items == nullptr) {  // the last queries have the most keys
-    const int first = (sh.pairs - 1 - pair) * kPair * c.tile_queries;
-    return Item{sh.one.q_row + first, min(sh.one.queries - first, kPair * c.tile_queries), sh.one.k_row, sh.one.pos + first};
-  }
+__device__ __forceinline__ Item load_item(const Params& c, int pair) {
   const int4 v = *reinterpret_cast<const int4*>(c.items + pair);
   return Item{v.x, v.y, v.z, v.w};
 }
@@ -158,8 +153,9 @@ __device__ __forceinline__ int claim(const Params& c) {
 }
 __device__ __forceinline__ void publish(const Params& c, Shared& sh, int item) {
   const int pair = item / c.kv_heads;
-  sh.work_head = pair < sh.pairs ? item - pair * c.kv_heads : -1;
-  if (pair < sh.pairs) sh.work = load_item(c, sh, pair);
+  const bool there = c.items != nullptr && pair < sh.pairs;  // without a list a CTA has one item
+  sh.work_head = there ? item - pair * c.kv_heads : -1;
+  if (there) sh.work = load_item(c, pair);
 }
 
 template <typename T>
@@ -302,19 +298,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     sh.abort = 0;
     sh.odd_values = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) {  // the CTA's first item
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the list of items is there
-    if (c.items == nullptr) {
-      int queries, keys;
-      span(c.query_start, 0, c.num_queries, sh.one.q_row, queries);
-      span(c.key_start, 0, c.num_keys, sh.one.k_row, keys);
-      sh.one.queries = queries, sh.one.pos = keys - queries;
-      sh.pairs = (queries + kPair * c.tile_queries - 1) / (kPair * c.tile_queries);
-      publish(c, sh, blockIdx.x);
-    } else {  // (all CTAs' first entries lie in the list's memory, used or not)
-      const int pair = blockIdx.x / c.kv_heads;
-      sh.work = load_item(c, sh, pair);
+    const int pair = blockIdx.x / c.kv_heads, head = blockIdx.x - pair * c.kv_heads;
+    if (c.items == nullptr) {  // no list: a lane per sequence
+      const int pair_queries = kPair * c.tile_queries;
+      int q_row = 0, queries = 0, k_row = 0, keys = 0;
+      if (lane < c.num_seqs) {
+        span(c.query_start, lane, c.num_queries, q_row, queries);
+        span(c.key_start, lane, c.num_keys, k_row, keys);
+      }
+      const int mine = (queries + pair_queries - 1) / pair_queries;
+      int upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += up;
+      }
+      if (pair < upto && pair >= upto - mine) {
+        const int first = (pair - (upto - mine)) * pair_queries;
+        sh.work = Item{q_row + first, min(queries - first, pair_queries), k_row, keys - queries + first};
+      }
+      if (lane == 31) sh.pairs = upto, sh.work_head = pair < upto ? head : -1;
+    } else if (lane == 0) {  // (all CTAs' first entries lie in the list's memory, used or not)
+      sh.work = load_item(c, pair);
       sh.pairs = *c.num_items;
-      sh.work_head = pair < sh.pairs ? blockIdx.x - pair * c.kv_heads : -1;
+      sh.work_head = pair < sh.pairs ? head : -1;
     }
   }
   if (warp == 2) {
@@ -965,10 +975,10 @@ extern "C" int cb_prompt_attention(const void* query, int64_t query_token_stride
   c.out = static_cast<char*>(out), c.out_ts = out_token_stride, c.out_hs = out_head_stride;
   c.error = device_error;
   c.query_start = query_start, c.key_start = key_start;
-  c.num_queries = static_cast<int>(num_queries), c.num_keys = static_cast<int>(num_keys);
-  // One sequence's items are an arithmetic series: no list, and one launch less (a 301-token prompt:
-  // 14.4 us with it).  Not where CTAs take several: the list kernel also clears their counter.
-  if (num_seqs > 1 || items * num_kv_heads > kSmCount) {
+  c.num_seqs = static_cast<int>(num_seqs), c.num_queries = static_cast<int>(num_queries), c.num_keys = static_cast<int>(num_keys);
+  // An item per CTA and a sequence per lane: each finds its own, and there is one launch less (4
+  // prompts of 300 tokens: 9.9 us, 12.5 with it).  Not where CTAs take several: the list kernel also clears their counter.
+  if (num_seqs > 32 || items * num_kv_heads > kSmCount) {
     int* num_items = static_cast<int*>(workspace);
     prompt::Item* list = reinterpret_cast<prompt::Item*>(static_cast<char*>(workspace) + 256);
     c.items = list, c.num_items = num_items;

@@ -148,6 +148,20 @@ def test_several_items_per_cta(cuda, lengths, keys):
     _check(got, q, k, v, starts.tolist(), key_starts.tolist(), 0.1)
 
 
+@pytest.mark.parametrize("lengths,keys,kv_heads", [
+    ([3, 0, 70, 1, 65], [3, 0, 70, 9, 200], 4),
+    ([1] * 32, [1, 130] * 16, 2),  # as many as a warp has lanes
+    ([1] * 33, [1, 130, 5] * 11, 2),
+    ([0, 0, 129, 0], [7, 0, 129, 0], 1),
+    ([130, 20, 0, 300], [0, 500, 0, 300], 2),
+])
+def test_few_items(cuda, lengths, keys, kv_heads):
+    q, k, v = _inputs(cuda, sum(lengths), sum(keys), 4 * kv_heads, kv_heads, 128, torch.float16, 12)
+    starts, key_starts = _starts(lengths, cuda), _starts(keys, cuda)
+    got = prompt_attention(q, k, v, starts, 0.09, key_start=key_starts)
+    _check(got, q, k, v, starts.tolist(), key_starts.tolist(), 0.09)
+
+
 def test_strides_and_rows_behind(cuda):
     """Slices of one projection's output; rows of no sequence stay as they were."""
     heads, kv_heads, head, tokens = 8, 2, 128, 333
