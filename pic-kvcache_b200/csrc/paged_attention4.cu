@@ -32,7 +32,7 @@
 //     movmatrix.  The roundings weigh with codes less 8, not with codes: 8 times the
 //     sum of the rounded factors (one more product, of ones) is taken off again and
 //     the low terms are taken at code 8, so that a row's offset does not multiply them
-//     (fp16 outputs of rows around 0: 3.4e-4 off without, 2.4e-4 with, 2.0e-4 for the
+//     (fp16 outputs of rows around 0: 3.4e-4 off without, 2.5e-4 with, 2.1e-4 for the
 //     rounding of the result alone).  M also carries the exponent of the largest
 //     step' so that a factor stays in fp16's range whatever the values' size: at most
 //     2^15, 2^10 when M is set.  M moves only when a factor would pass that, which each
