@@ -97,7 +97,9 @@ class PagedKV4:
 
 
 _HERE = contextlib.nullcontext()
-_raw_stream = torch._C._cuda_getCurrentRawStream  # no Stream object is built (2 us of a decode call)
+# No Stream object is built (2 us of a decode call).  None on a torch without CUDA bindings, where every
+# call refuses its tensors before it needs a stream.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def on_device(device: int, stream: torch.cuda.Stream | None):

@@ -100,3 +100,25 @@ def test_c_entry_4_bit_refuses():
     assert lib.cb_gather_paged_kv4(*[None, None, 0, 0, 0, None, None, 0, 0, 0, 4, 16, 2, 64, None, 1, None, 0, 0, 0, 0, None]) == \
         _native.CB_ERR_INVALID
     assert isinstance(lib.cb_gather_paged_kv4, ctypes._CFuncPtr)
+
+
+def test_import_without_cuda_bindings():
+    """The package imports, and refuses CPU tensors as ever, on a torch that has no CUDA bindings."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import torch
+for name in [n for n in dir(torch._C) if n.startswith("_cuda_")]:
+    delattr(torch._C, name)
+from cacheblend_b200 import CacheBlendConfig, append_paged_kv, paged_attention4
+key, pages = torch.zeros(3, 2, 64), torch.zeros(2, 4, 16, 2, 64)
+try:
+    append_paged_kv(None, None, key, key, pages, torch.arange(3), 16)
+except RuntimeError as error:
+    print(error)
+"""
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True,
+                         cwd=Path(__file__).resolve().parents[1] / "pic-kvcache_b200")
+    assert run.returncode == 0 and "CUDA tensors only" in run.stdout, run.stderr
