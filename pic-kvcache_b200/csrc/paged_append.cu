@@ -562,7 +562,8 @@ __global__ void __launch_bounds__(kThreads) append4_kernel(const Params c) {
       for (int o = D / 32; o >= 1; o >>= 1) ends[s] = Two<T>::least(ends[s], __shfl_xor_sync(0xffffffffu, ends[s], o));
       const float2 e = Two<T>::open(ends[s]);
       far[s] = !(fmaxf(-e.x, -e.y) <= kHalfMax);
-      pair[s] = step_of(e.x, -e.y, !(fabsf(e.x) + fabsf(e.y) < INFINITY));
+      // (each end by itself: the sum of two finite ones may pass fp32)
+      pair[s] = step_of(e.x, -e.y, !(fabsf(e.x) < INFINITY && fabsf(e.y) < INFINITY));
     }
     if constexpr (D == 64) pair[1] = pair[0], far[1] = far[0];
     if (is_q || !g.stored || w.head + i >= heads) continue;

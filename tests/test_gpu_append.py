@@ -313,3 +313,18 @@ def test_append_streams_and_graph(cuda):
     torch.cuda.synchronize()
     assert torch.equal(pages, want) and torch.equal(in_graph, turned) and torch.equal(cache.codes, cache_want.codes)
     assert torch.equal(read, gather_paged_kv4(cache_want, slots))
+
+
+@pytest.mark.parametrize("pad", [0, 1], ids=["aligned", "unaligned"])
+def test_4_bit_groups_at_the_ends_of_bf16(cuda, pad):
+    """Finite groups whose ends add up to more than fp32 holds: held at fp16's end, not NaN."""
+    top = torch.finfo(torch.bfloat16).max
+    x = torch.ones(4, 1, 128 + pad, dtype=torch.bfloat16, device=cuda)[..., pad:]
+    x[0], x[1], x[2], x[2, 0, ::2], x[3, 0, :64] = -top, top, top, -top, -2e38
+    cache = PagedKV4.allocate(1, 4, 1, 128, cuda)
+    append_paged_kv4(None, None, x, x, cache, torch.arange(4, device=cuda))
+    want = torch.ones(4, 1, 128, device=cuda)
+    want[0], want[1], want[3, 0, :64] = -65504, 65504, -65504
+    want[2], want[2, 0, ::2] = 15 * 8736 - 65504, -65504  # a step of fp16(131008 / 15) = 8736
+    got = gather_paged_kv4(cache, torch.arange(4, device=cuda), torch.float32)
+    assert torch.equal(got[0], want) and torch.equal(got[1], want)
