@@ -116,7 +116,8 @@ struct Params {
 
 // One sequence's share of the line.
 struct Seq {
-  int first_token, tokens, len;
+  int first_token, tokens;
+  int len, before;                // keys that the table has room for; those before the query tokens, past it or not
   int row_blocks, tiles, rounds;  // tiles and rounds per piece
   int64_t work;                   // of all its pieces
 };
@@ -129,7 +130,9 @@ __device__ __forceinline__ Seq sequence(const Params& c, int i) {
   s.first_token = static_cast<int>(a);
   s.tokens = static_cast<int>(b - a);
   const int64_t most = static_cast<int64_t>(c.width) * c.block_size;
-  s.len = static_cast<int>(min(static_cast<int64_t>(max(__ldg(c.lens + i), 0)), most));
+  const int all = max(__ldg(c.lens + i), 0);
+  s.len = static_cast<int>(min(static_cast<int64_t>(all), most));
+  s.before = all - s.tokens;
   s.row_blocks = static_cast<int>((static_cast<int64_t>(s.tokens) * c.groups + kRows - 1) / kRows);
   s.tiles = max(1, (s.len + kTileKeys - 1) / kTileKeys);
   s.rounds = (s.tiles + kRound - 1) / kRound;
@@ -233,6 +236,7 @@ struct Walk {
 };
 struct Piece {
   int seq, head, row0, tile0, tile1, len, tokens, first_token;  // tile1 < 0: the share is done
+  int before;
   bool whole;
 };
 __device__ __noinline__ void next_piece(const Params& c, Walk& walk, Piece& piece) {
@@ -259,6 +263,7 @@ __device__ __noinline__ void next_piece(const Params& c, Walk& walk, Piece& piec
     piece.tile0 = max(from - kPieceCost, 0) * kRound;
     piece.tile1 = min((to - kPieceCost) * kRound, s.tiles);
     piece.len = s.len, piece.tokens = s.tokens, piece.first_token = s.first_token;
+    piece.before = s.before;
     piece.whole = piece.tile0 == 0 && piece.tile1 == s.tiles;
     if (piece.tile0 == 0 && !piece.whole)
       c.meta[blockIdx.x] = Cut{static_cast<int>((length - to + walk.share - 1) / walk.share), piece.head, piece.row0,
@@ -333,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention4_kernel(const __grid_co
     if (tile1 < 0) break;
     const int head = piece.head, row0 = piece.row0;
     // the fewest keys that any row of the piece sees
-    const int all_see = piece.len - piece.tokens + row0 / c.groups + 1;
+    const int all_see = piece.before + row0 / c.groups + 1;
 
     // ---- the pipeline of this warp's tiles: the next table entry is always on its way
     const int32_t* table = c.table + static_cast<int64_t>(piece.seq) * c.table_stride;
@@ -462,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention4_kernel(const __grid_co
     for (int j = 0; j < 2; ++j) {
       const int col = 2 * t + j;
       factor[j] = __shfl_sync(0xffffffffu, f, col * 4);
-      last[j] = len - piece.tokens + min(row0 + col, piece.tokens * c.groups - 1) / c.groups;
+      last[j] = piece.before + min(row0 + col, piece.tokens * c.groups - 1) / c.groups;
     }
 
     float o[kChunks][2][4], eights[4], low[kGroups][2], m[2], l[2];

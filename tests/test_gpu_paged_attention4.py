@@ -292,3 +292,16 @@ def test_append_then_attend(cuda):
         got = paged_attention4(query, cache, table, lens, head ** -0.5)
         _check(got, query, cache, table, lens.tolist(), head ** -0.5)
     assert gather_paged_kv4(cache, table[0, :1].long() * block).isfinite().all()
+
+
+@pytest.mark.parametrize("length,count", [(200, 3), (130, 5), (129, 2)])
+def test_several_tokens_of_a_length_past_the_table(cuda, length, count):
+    """Keys past the table's width are left out; which of the rest a token sees goes by the whole length."""
+    cache, table = _pages(cuda, [200], 16, 2, 128, 14)
+    table = table[:, :8].contiguous()  # 128 keys
+    query = torch.randn(count, 8, 128, device=cuda, generator=torch.Generator(device=cuda).manual_seed(1)).to(torch.bfloat16)
+    got = paged_attention4(query, cache, table, torch.tensor([length], dtype=torch.int32, device=cuda), 128 ** -0.5,
+                           query_start=torch.tensor([0, count], dtype=torch.int32, device=cuda))
+    seen = [min(length - count + j + 1, 128) for j in range(count)]
+    assert bool(got.isfinite().all())
+    _check(got, query, cache, table.expand(count, -1), seen, 128 ** -0.5)
