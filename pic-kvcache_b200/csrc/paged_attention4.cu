@@ -33,10 +33,10 @@
 //     sum of the rounded factors (one more product, of ones) is taken off again and
 //     the low terms are taken at code 8, so that a row's offset does not multiply them
 //     (fp16 outputs of rows around 0: 3.4e-4 off without, 2.5e-4 with, 2.1e-4 for the
-//     rounding of the result alone).  M also carries the exponent of the largest
-//     step' so that a factor stays in fp16's range whatever the values' size: at most
-//     2^15, 2^10 when M is set.  M moves only when a factor would pass that, which each
-//     lane sees for itself: the common tile needs no maximum over the warp.
+//     rounding of the result alone).  M is taken over p step' of the keys that a
+//     row sees, so that a factor stays in fp16's range whatever the values' size: at most
+//     2^15, and the largest 2^10 when M is set.  M moves only when a factor would pass that,
+//     which each lane bounds for itself: the common tile needs no maximum over the warp.
 // Sums, maxima, steps and the low terms are fp32.
 //
 // Memory: a warp takes tiles of 32 keys of one KV head through a ring of its
@@ -546,15 +546,26 @@ __global__ void __launch_bounds__(kThreads, 2) attention4_kernel(const __grid_co
       // steps below 2^-24 do not exist in fp16, but rows of step 0 do
       const float room = lg2(fmaxf(__low2float(most), 5.9604645e-8f));
 
-      // ---- the reference M moves only when a factor would pass 2^15
+      // ---- the reference M moves only when a factor would pass 2^15: the largest logit with the largest
+      // step is a bound on them
       bool move = false;
-      float top[2];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        top[j] = fmaf(fmaxf(fmaxf(w[0][j], w[0][j + 2]), fmaxf(w[1][j], w[1][j + 2])), factor[j], room);
-        move |= top[j] > m[j] + kMostRoom;
-      }
+      for (int j = 0; j < 2; ++j)
+        move |= fmaf(fmaxf(fmaxf(w[0][j], w[0][j + 2]), fmaxf(w[1][j], w[1][j + 2])), factor[j], room) > m[j] + kMostRoom;
       if (__any_sync(0xffffffffu, move)) {
+        // M goes by the factors themselves: set by the bound, a large step of a key that hardly weighs, or
+        // that the row does not see, would take the bits of those that do
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            __half2 step = __habs2(*reinterpret_cast<const __half2*>(&vpair[mt][r][0]));
+            if constexpr (kGroups == 2) step = __hmax2(step, __habs2(*reinterpret_cast<const __half2*>(&vpair[mt][r][kGroups - 1])));
+            const float own = lg2(fmaxf(__low2float(step), 5.9604645e-8f));
+#pragma unroll
+            for (int j = 0; j < 2; ++j) top[j] = fmaxf(top[j], fmaf(w[mt][r * 2 + j], factor[j], own));
+          }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           float high = top[j];

@@ -305,3 +305,43 @@ def test_several_tokens_of_a_length_past_the_table(cuda, length, count):
     seen = [min(length - count + j + 1, 128) for j in range(count)]
     assert bool(got.isfinite().all())
     _check(got, query, cache, table.expand(count, -1), seen, 128 ** -0.5)
+
+
+@pytest.mark.parametrize("head", [64, 128])
+@pytest.mark.parametrize("step", [math.inf, 65504.0, 1e-7])
+def test_steps_that_a_row_does_not_see(cuda, head, step):
+    """The step of a later token's V row changes no bit of the tokens before it."""
+    lens, start = [123], torch.tensor([0, 3], dtype=torch.int32, device=cuda)
+    cache, table = _pages(cuda, lens, 16, 1, head, 9)
+    query = torch.randn(3, 2, head, device=cuda, generator=torch.Generator(device=cuda).manual_seed(1)).to(torch.float16)
+    lengths = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    clean = paged_attention4(query, cache, table, lengths, head ** -0.5, query_start=start)
+    cache.scales[1, table[0, 7], 0, 10, 0, 0] = step  # key 122
+    got = paged_attention4(query, cache, table, lengths, head ** -0.5, query_start=start)
+    assert torch.equal(got[:2], clean[:2])
+    assert bool(got[:2].isfinite().all())
+    if step < 1:
+        assert bool(got.isfinite().all())
+        _check(got, query, cache, table, lens, head ** -0.5, [0, 3])
+
+
+@pytest.mark.parametrize("head", [64, 128])
+def test_rows_of_very_different_step(cuda, head):
+    """V rows of large step that hardly weigh take no bits of those that do.
+
+    Two keys have a logit of 60, the others of -60, and a key in 32, of the latter, has a V row of step 4,000
+    where the rest have about 2e-6.  The reference keeps the largest factor p step' over 2^10, so fp16
+    subnormals (off by 2^-25) are off by 2^-35 of the largest p step' at most: the term of _check covers
+    them, as long as p and step' are taken from the same key."""
+    n = 500
+    cache, table = _pages(cuda, [n], 16, 2, head, 15, step=(1e-6, 4e-6), low=(-2e-5, 2e-5))
+    at = torch.arange(3, n, 32, device=cuda)
+    page, row = table[0].long()[at // 16], at % 16
+    cache.scales[1, page, :, row, :, 0], cache.scales[1, page, :, row, :, 1] = 4000.0, -20000.0
+    cache.scales[0, ..., 0], cache.scales[0, ..., 1] = 0.0, -1.0
+    for key in (11, 331):  # beside keys 3 and 323 in a lane
+        cache.scales[0, table[0, key // 16], :, key % 16, :, 1] = 1.0
+    query = torch.ones(1, 8, head, device=cuda, dtype=torch.bfloat16)
+    got = paged_attention4(query, cache, table, torch.tensor([n], dtype=torch.int32, device=cuda), 60.0 / head)
+    assert bool(got.isfinite().all())
+    _check(got, query, cache, table, [n], 60.0 / head)
