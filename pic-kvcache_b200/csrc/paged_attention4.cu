@@ -194,6 +194,11 @@ __device__ __forceinline__ float lg2(float x) {
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
 __device__ __forceinline__ uint32_t pack(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -483,8 +488,9 @@ __global__ void __launch_bounds__(kThreads, 2) attention4_kernel(const __grid_co
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[ch][i][j] = 0.0f;
 
-    // a tile; CUT: some row does not see some key of it
-    auto consume = [&](auto cut_tag, int key0, uint32_t buf, uint32_t mask) {
+    // a tile; CUT: some row does not see some key of it, or a step is not finite, which without CUT
+    // is found before anything has changed (false)
+    auto consume = [&](auto cut_tag, int key0, uint32_t buf, uint32_t mask) -> bool {
       constexpr bool CUT = decltype(cut_tag)::value;
       const uint32_t rows_at = buf + L::where(lane & 15, lane >> 4);
       const uint32_t pairs_at = buf + 2 * L::kCodes + g * 2 * L::kPairs;
@@ -508,9 +514,13 @@ __global__ void __launch_bounds__(kThreads, 2) attention4_kernel(const __grid_co
           lows[r] = kGroups == 2 ? __byte_perm(pair[r][0], pair[r][kGroups - 1], 0x7632) : pair[r][0] >> 16;
 #pragma unroll
           for (int G = 0; G < kGroups; ++G) {
-            if constexpr (CUT)
+            if constexpr (CUT) {
               if (!((mask >> (mt * 16 + r * 8 + g)) & 1u)) vpair[mt][r][G] = 0;
-            most = __hmax2(most, __habs2(*reinterpret_cast<const __half2*>(&vpair[mt][r][G])));
+              // A group whose step is not finite goes by its lowest value alone, made NaN: a factor of NaN
+              // would meet the other group's zeros in the sums of factors, an infinite one would set M.
+              if ((vpair[mt][r][G] & 0x7c00u) == 0x7c00u) vpair[mt][r][G] = 0x7e000000u;
+            }
+            most = __hmax2_nan(most, __habs2(*reinterpret_cast<const __half2*>(&vpair[mt][r][G])));
           }
         }
         float acc[kGroups][4];
@@ -544,15 +554,17 @@ __global__ void __launch_bounds__(kThreads, 2) attention4_kernel(const __grid_co
         }
       }
       // steps below 2^-24 do not exist in fp16, but rows of step 0 do
-      const float room = lg2(fmaxf(__low2float(most), 5.9604645e-8f));
+      const float room = lg2(max_nan(__low2float(most), 5.9604645e-8f));
 
       // ---- the reference M moves only when a factor would pass 2^15: the largest logit with the largest
-      // step is a bound on them
-      bool move = false;
+      // step is a bound on them (NaN where a step is, which counts as passed)
+      bool stay = true;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
-        move |= fmaf(fmaxf(fmaxf(w[0][j], w[0][j + 2]), fmaxf(w[1][j], w[1][j + 2])), factor[j], room) > m[j] + kMostRoom;
-      if (__any_sync(0xffffffffu, move)) {
+        stay &= fmaf(fmaxf(fmaxf(w[0][j], w[0][j + 2]), fmaxf(w[1][j], w[1][j + 2])), factor[j], room) <= m[j] + kMostRoom;
+      if (!__all_sync(0xffffffffu, stay)) {
+        if constexpr (!CUT)
+          if (!__all_sync(0xffffffffu, room < INFINITY)) return false;
         // M goes by the factors themselves: set by the bound, a large step of a key that hardly weighs, or
         // that the row does not see, would take the bits of those that do
         float top[2] = {-INFINITY, -INFINITY};
@@ -630,6 +642,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention4_kernel(const __grid_co
           mma(eights, G == 0 ? kEight : 0u, G == 0 ? 0u : kEight, G == 0 ? kEight : 0u, G == 0 ? 0u : kEight, b[G][0], b[G][1]);
         }
       }
+      return true;
     };
 
     int stage = 0;
@@ -640,10 +653,8 @@ __global__ void __launch_bounds__(kThreads, 2) attention4_kernel(const __grid_co
       const uint32_t buf = ring_at + stage * L::kBytes;
       const uint32_t mask = live[warp][stage];
       const int key0 = tile * kTileKeys;
-      if (mask != 0xffffffffu || key0 + kTileKeys > all_see)
+      if (mask != 0xffffffffu || key0 + kTileKeys > all_see || !consume(std::false_type{}, key0, buf, mask))
         consume(std::true_type{}, key0, buf, mask);
-      else
-        consume(std::false_type{}, key0, buf, mask);
       __syncwarp();  // the stage may be filled again
       stage = stage + 1 == kStages ? 0 : stage + 1;
     }

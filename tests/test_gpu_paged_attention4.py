@@ -345,3 +345,22 @@ def test_rows_of_very_different_step(cuda, head):
     got = paged_attention4(query, cache, table, torch.tensor([n], dtype=torch.int32, device=cuda), 60.0 / head)
     assert bool(got.isfinite().all())
     _check(got, query, cache, table, [n], 60.0 / head)
+
+
+@pytest.mark.parametrize("step", [math.nan, math.inf])
+@pytest.mark.parametrize("group", [0, 1])
+@pytest.mark.parametrize("key", [5, 995])  # in a whole tile, in the last one
+def test_not_finite_keeps_to_its_group(cuda, step, group, key):
+    """A V row's group that is not finite reaches its own 64 dimensions, in the rows that see it."""
+    lens, heads, head = [1000, 77], 8, 128
+    cache, table = _pages(cuda, lens, 16, 2, head, 16)
+    query = torch.randn(2, heads, head, device=cuda, generator=torch.Generator(device=cuda).manual_seed(1)).to(torch.bfloat16)
+    lengths = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    clean = paged_attention4(query, cache, table, lengths, head ** -0.5)
+    bad = PagedKV4(cache.codes, cache.scales.clone())
+    bad.scales[1, table[0, key // 16], 0, key % 16, group, 0] = step  # KV head 0: query heads 0 to 3
+    got = paged_attention4(query, bad, table, lengths, head ** -0.5)
+    hit = torch.zeros(2, heads, head, dtype=torch.bool, device=cuda)
+    hit[0, :4, 64 * group:64 * group + 64] = True
+    assert not bool(got[hit].isfinite().any()) and bool(got[~hit].isfinite().all())
+    _check(torch.where(hit, clean, got), query, cache, table, lens, head ** -0.5)
