@@ -81,6 +81,9 @@ constexpr int kUncutKeys = 2 * kRound * kTileKeys;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSetRoom = 10.0f;   // a factor p step' is at most 2^10 when M is set,
 constexpr float kMostRoom = 15.0f;  // and 2^15 before M moves
+// Logits below this count as this when M is set: a row that sees a key has a finite M, so that one of
+// which no weight is left (fp32 does not hold its logits) ends as 0 / 0 and not as a row without keys.
+constexpr float kLeast = -3e38f;
 
 // A piece that a CTA began and others go on with.
 struct alignas(32) Cut {
@@ -557,11 +560,11 @@ __global__ void __launch_bounds__(kThreads, 2) attention4_kernel(const __grid_co
       const float room = lg2(max_nan(__low2float(most), 5.9604645e-8f));
 
       // ---- the reference M moves only when a factor would pass 2^15: the largest logit with the largest
-      // step is a bound on them (NaN where a step is, which counts as passed)
+      // step is a bound on them (NaN where a step is, which counts as passed, as -inf does while there is no M)
       bool stay = true;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
-        stay &= fmaf(fmaxf(fmaxf(w[0][j], w[0][j + 2]), fmaxf(w[1][j], w[1][j + 2])), factor[j], room) <= m[j] + kMostRoom;
+        stay &= fmaf(fmaxf(fmaxf(w[0][j], w[0][j + 2]), fmaxf(w[1][j], w[1][j + 2])), factor[j], room) < m[j] + kMostRoom;
       if (!__all_sync(0xffffffffu, stay)) {
         if constexpr (!CUT)
           if (!__all_sync(0xffffffffu, room < INFINITY)) return false;
@@ -576,7 +579,8 @@ __global__ void __launch_bounds__(kThreads, 2) attention4_kernel(const __grid_co
             if constexpr (kGroups == 2) step = __hmax2(step, __habs2(*reinterpret_cast<const __half2*>(&vpair[mt][r][kGroups - 1])));
             const float own = lg2(fmaxf(__low2float(step), 5.9604645e-8f));
 #pragma unroll
-            for (int j = 0; j < 2; ++j) top[j] = fmaxf(top[j], fmaf(w[mt][r * 2 + j], factor[j], own));
+            for (int j = 0; j < 2; ++j)
+              if (!CUT || w[mt][r * 2 + j] != -INFINITY) top[j] = fmaxf(top[j], fmaxf(fmaf(w[mt][r * 2 + j], factor[j], own), kLeast));
           }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -713,7 +717,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention4_kernel(const __grid_co
         value.y = fmaf(y.y + add, by, value.y);
       }
       if (whole) {
-        const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;  // a row that sees no key is zeros
+        const float inverse = top == -INFINITY ? 0.0f : 1.0f / sum;  // a row that sees no key is zeros
         const int r = row0 + row, token = r / c.groups;
         QT* dst = reinterpret_cast<QT*>(c.out + (piece.first_token + static_cast<int64_t>(token)) * c.out_ts +
                                         static_cast<int64_t>(head * c.groups + r - token * c.groups) * c.out_hs) + dim;
@@ -793,7 +797,7 @@ __global__ void __launch_bounds__(kThreads) join4_kernel(const Params c) {
     const int token = r / c.groups;
     QT* dst = reinterpret_cast<QT*>(c.out + (cut.first_token + static_cast<int64_t>(token)) * c.out_ts +
                                     static_cast<int64_t>(cut.head * c.groups + r - token * c.groups) * c.out_hs) + d;
-    *dst = Elem<QT>::from_f(l == 0.0f ? 0.0f : v / l);
+    *dst = Elem<QT>::from_f(all == -INFINITY ? 0.0f : v / l);
   }
 }
 

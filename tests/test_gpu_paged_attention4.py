@@ -364,3 +364,28 @@ def test_not_finite_keeps_to_its_group(cuda, step, group, key):
     hit[0, :4, 64 * group:64 * group + 64] = True
     assert not bool(got[hit].isfinite().any()) and bool(got[~hit].isfinite().all())
     _check(torch.where(hit, clean, got), query, cache, table, lens, head ** -0.5)
+
+
+@pytest.mark.parametrize("size", [2.0 ** 105, 2.0 ** 118, torch.finfo(torch.bfloat16).max])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_logits_past_fp32(cuda, size, sign):
+    """Logits that fp32 does not tell apart, or does not hold: the value of the highest, or not finite -- never
+    the zeros of a row that sees no key, and the same in whole tiles and in cut ones."""
+    lens, best = [20, 64, 1100, 0], (7, 40, 1030)
+    cache, table = _pages(cuda, lens, 16, 2, 128, 17)
+    cache.scales[0, ..., 0], cache.scales[0, ..., 1] = 0.0, 1.0  # rows of K that are 1 throughout, one of them 1 +- 1/2
+    for i, key in enumerate(best):
+        cache.scales[0, table[i, key // 16], :, key % 16, :, 1] = 1.0 + 0.5 * sign
+    query = torch.full((4, 8, 128), sign * size, device=cuda, dtype=torch.bfloat16)
+    got = paged_attention4(query, cache, table, torch.tensor(lens, dtype=torch.int32, device=cuda), 1.0)
+    assert int((got[3] != 0).sum()) == 0
+    u = torch.finfo(query.dtype).eps / 2
+    for i, key in enumerate(best):
+        varied, low = (x[key].repeat_interleave(4, 0) for x in _parts(cache, table[i], lens[i], 1))
+        # one factor p step rounded to fp16, and the result
+        off, bound = (got[i].double() - varied - low).abs(), u * (varied + low).abs() + (2.0 ** -11 + 2.0 ** -20) * (varied + low.abs())
+        assert bool(((off <= bound) | ~got[i].isfinite()).all())
+    # several tokens, the first of which sees nothing
+    got = paged_attention4(query[:3], cache, table[:1], torch.tensor([2], dtype=torch.int32, device=cuda), 1.0,
+                           query_start=torch.tensor([0, 3], dtype=torch.int32, device=cuda))
+    assert int((got[0] != 0).sum()) == 0 and bool((got[1:] != 0).any(-1).all())
