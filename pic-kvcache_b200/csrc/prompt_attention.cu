@@ -720,7 +720,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the P V of the item's boundary tiles came after their look-through
       const bool odd = *reinterpret_cast<volatile int*>(&sh.odd_values) != 0;
       const bool seen = n > 0 && pos >= 0;
-      const float inv = l != 0.0f ? __fdividef(1.0f, l) : 0.0f;  // (2 ulp at most)
+      // (2 ulp at most.)  A row that sees no key is zeros; one that does, and of whose logits no weight is
+      // left (all -inf), 0 / 0.
+      const float inv = pos >= 0 ? __fdividef(1.0f, l) : 0.0f;
       // A row per thread, so a store of 16 bytes each would touch 32 lines (47 cycles of the load/store
       // unit, 6,000 for the item's two tiles, with the other warps' loads behind them).  The packed
       // rows go back to TMEM, over O, and come again as (row, 16 bytes) by lane / 4 and lane % 4:

@@ -275,3 +275,21 @@ def test_long_prompt(cuda):
     want, bound = _want(q[8900:], k, v, 128 ** -0.5)
     bound += want.abs() * 2.0 ** -8 + 1e-30
     assert float(((got[8900:].double() - want).abs() / bound).max()) <= 1
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("head", [64, 128])
+def test_logits_of_minus_infinity(cuda, dtype, head):
+    """A row whose seen logits are all -inf is NaN, as of any softmax of them; beside a finite one they weigh
+    nothing; a row that sees no key is zeros."""
+    q, k, v = _inputs(cuda, 300 + 200 + 40, 300 + 200, 8, 2, head, dtype, 13)
+    q[..., 0] = 1.0
+    k[:300, :, 0] = -torch.inf
+    k[100, :, 0] = 0.0  # the only finite logit of the first sequence
+    start, key_start = _starts([300, 200, 40], cuda), _starts([300, 200, 0], cuda)
+    got = prompt_attention(q, k, v, start, 0.1, key_start=key_start)
+    assert bool(got[:100].isnan().all())
+    assert torch.equal(got[100:300], v[100].repeat_interleave(4, 0).expand(200, -1, -1))
+    assert int((got[500:] != 0).sum()) == 0
+    assert bool(got[100:].isfinite().all())
+    _check(got[300:500], q[300:500], k[300:], v[300:], [0, 200], [0, 200], 0.1)
