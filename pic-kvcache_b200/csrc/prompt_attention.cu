@@ -7,8 +7,8 @@
 //   out = softmax(scale q k^T over the seen keys) v,  head h on KV head h / groups
 // Logits, softmax and sums are fp32; the unnormalized probabilities are rounded
 // to the element type for the second product (2^-8 bf16, 2^-11 fp16, relative,
-// each its own: about what rounding the output costs), and O is divided by the
-// fp32 row sum at the end.
+// each its own: about what rounding the output costs; an fp16 one below 2^-21 of the
+// largest is off by 2^-32 of that instead), and O is divided by the fp32 row sum at the end.
 //
 // Rows are (query, group) pairs of one KV head, so a K / V tile serves the whole
 // group; a tile is 128 / groups queries (the last rows of a tile whose group
@@ -33,7 +33,7 @@
 // softmax the tensor cores have the other's two products.  P is handed over in
 // two halves, and P V begins on the first.
 // O is rescaled only when a row's maximum grows by more than 2^8 (until then the
-// stale one keeps every exp2 <= 256); that P V (t - 1) is finished is known from
+// stale one keeps every exp2 <= 2^8, or 2^15 in fp16); that P V (t - 1) is finished is known from
 // S (t), which was issued behind it.
 //
 // Masked places: a logit that a row does not see is replaced, whatever it is.  A
@@ -72,6 +72,11 @@ constexpr int kRegsControl = 56;
 constexpr int kRegsSoftmax = 224;
 static_assert(4 * 32 * kRegsControl + 8 * 32 * kRegsSoftmax <= kThreads * 168, "register split");
 constexpr float kRescaleLog2 = 8.0f;
+// Where the reference is set, below the row's maximum: an fp16 probability is then 2^7 there (2^15 at most
+// before the reference moves), so that fp16's subnormals, 2^-25 off, are 2^-32 of the largest and not
+// 2^-25, which over the keys of a long context would be more than the rounding of the result.
+template <typename T>
+constexpr float kSetLog2 = std::is_same<T, __half>::value ? 7.0f : 0.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // One pair of query tiles of one sequence (for every KV head).
@@ -622,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto last_reader = [&](int kt) { return x == 1 || kt >= n_b; };
       const bool store = query_in_tile < tile_valid(c, w, x);
       const int pos = w.pos + x * c.tile_queries + query_in_tile;  // the last key this row sees
-      float m_used = -INFINITY;  // log2-domain maximum the exponentials are taken against
+      float m_used = -INFINITY;  // what the exponentials are taken against, in the log2 domain
       float l = 0.0f;
       // whole tiles: up to the last key that the warp's first row sees
       const int first_pos = w.pos + first_query;
@@ -656,9 +661,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int j = 4; j < 64; ++j) mx[j & 3] = max3(mx[j & 3], s_of(2 * j), s_of(2 * j + 1));
         const float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c.scale_log2;
-        const bool grow = tile_max > m_used + kRescaleLog2 || (m_used == -INFINITY && tile_max > -INFINITY);
+        const bool grow = tile_max > m_used + (kSetLog2<T> + kRescaleLog2) || (m_used == -INFINITY && tile_max > -INFINITY);
         if (__any_sync(0xffffffffu, grow)) {
-          const float m_new = grow ? tile_max : m_used;
+          const float m_new = grow ? tile_max - kSetLog2<T> : m_used;
           const float corr = grow ? (m_used == -INFINITY ? 0.0f : ex2(m_used - m_new)) : 1.0f;
           if (kt > 0) {  // O holds earlier tiles of this item, all finished: rescale its rows
 #pragma unroll 1

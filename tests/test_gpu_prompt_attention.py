@@ -293,3 +293,24 @@ def test_logits_of_minus_infinity(cuda, dtype, head):
     assert int((got[500:] != 0).sum()) == 0
     assert bool(got[100:].isfinite().all())
     _check(got[300:500], q[300:500], k[300:], v[300:], [0, 200], [0, 200], 0.1)
+
+
+@pytest.mark.parametrize("last", [False, True], ids=["peak first", "peak last"])
+def test_small_fp16_probabilities(cuda, last):
+    """Many keys of small weight beside one of large weight and value 0.
+
+    Their probabilities, 2^-25.2 of the largest, are what the output consists of.  An fp16 probability of
+    2^7 2^-25.2 (the reference lies 2^7 below the maximum, or more where a later one is larger) is a subnormal,
+    off by 2^-25 at most: n keys by n 2^-32 max |v|, against an output of n 2^-25.2.  The logits are exact
+    (one dimension, multiples of 2^-4); exp2 and the sums as in the bound above."""
+    n, head = 4096, 128
+    q, k, v = (torch.zeros(m, 1, head, dtype=torch.float16, device=cuda) for m in (1, n + 1, n + 1))
+    q[..., 0], k[..., 0] = 1.0, -25.1875
+    k[n if last else 0, :, 0] = 0.0
+    v[:] = 1.0
+    v[n if last else 0] = 0.0
+    scale = math.log(2.0)  # logits as powers of two
+    got = prompt_attention(q, k, v, _starts([1], cuda), scale, key_start=_starts([n + 1], cuda))
+    want, _ = _want(q, k, v, scale)
+    off = (got.double() - want).abs()
+    assert float((off / (want * (2.0 ** -11 + 2.0 ** -15 * 27) + (n + 1) * 2.0 ** -32)).max()) <= 1
