@@ -287,8 +287,6 @@ def prompt_attention(
         result = _attention_out(query, out)
         if tokens == 0 or seqs == 0:
             return result
-        if keys == 0:
-            raise ValueError("prompt attention needs keys")
         workspace = _scratch(
             workspace, lambda: _prompt_bytes(tokens, seqs, heads, kv_heads, head_size), query.device)
         strides = (*strides, result.stride())

@@ -942,7 +942,7 @@ extern "C" int cb_prompt_attention(const void* query, int64_t query_token_stride
   CB_REQUIRE(scale > 0.0f, "the scale must be positive (got %g)", static_cast<double>(scale));
   if (num_queries == 0 || num_seqs == 0) return CB_OK;
   CB_REQUIRE(query && query_start && key_start && out && workspace, "null pointer argument");
-  CB_REQUIRE(num_keys > 0 && key && value, "prompt attention needs keys and values");
+  CB_REQUIRE(num_keys == 0 || (key && value), "null key or value pointer");
   const uint64_t acc = reinterpret_cast<uint64_t>(query) | reinterpret_cast<uint64_t>(key) |
                        reinterpret_cast<uint64_t>(value) | reinterpret_cast<uint64_t>(out) | (uint64_t)query_token_stride |
                        (uint64_t)query_head_stride | (uint64_t)key_token_stride | (uint64_t)key_head_stride |
@@ -967,10 +967,11 @@ extern "C" int cb_prompt_attention(const void* query, int64_t query_token_stride
     rc = tc::encode_4d(encode, &q_map, dtype, query, dims, strides, static_cast<uint32_t>(groups), 1,
                        static_cast<uint32_t>(tile_queries));
   }
-  if (rc == CB_OK)
+  if (num_keys == 0) k_map = v_map = q_map;  // every row is zeros, and neither map is used
+  if (rc == CB_OK && num_keys > 0)
     rc = tc::encode_3d(encode, &k_map, dtype, key, head_size, num_kv_heads, num_keys, key_head_stride, key_token_stride, 1,
                        tc::kTile);
-  if (rc == CB_OK)
+  if (rc == CB_OK && num_keys > 0)
     rc = tc::encode_3d(encode, &v_map, dtype, value, head_size, num_kv_heads, num_keys, value_head_stride,
                        value_token_stride, 1, tc::kTile);
   if (rc != CB_OK) return rc;

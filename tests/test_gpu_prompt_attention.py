@@ -314,3 +314,14 @@ def test_small_fp16_probabilities(cuda, last):
     want, _ = _want(q, k, v, scale)
     off = (got.double() - want).abs()
     assert float((off / (want * (2.0 ** -11 + 2.0 ** -15 * 27) + (n + 1) * 2.0 ** -32)).max()) <= 1
+
+
+def test_no_keys_at_all(cuda):
+    """Zeros in the rows of the sequences, the rest as it was."""
+    q, k, v = _inputs(cuda, 90, 0, 4, 2, 64, torch.bfloat16, 14)
+    for lengths in ([40, 45], [1] * 40):  # found by the CTAs themselves, and from a list
+        out = torch.full_like(q, 3.0)
+        starts = _starts(lengths, cuda, first=2)
+        got = prompt_attention(q, k, v, starts, 0.125, key_start=torch.zeros_like(starts), out=out)
+        end = 2 + sum(lengths)
+        assert int((got[2:end] != 0).sum()) == 0 and bool((got[:2] == 3).all()) and bool((got[end:] == 3).all())
