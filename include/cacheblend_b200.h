@@ -485,7 +485,8 @@ CB_API int cb_append_paged_kv4(const void* key, int64_t key_token_stride, int64_
 
 /*
  * Rows of 4-bit pages as values: out[plane, t] = the row of slots[t], rounded
- * once to `dtype`; zeros for a slot outside the cache (padding).
+ * once to `dtype` (fp16: finite values past its end are held there); zeros for a slot outside the
+ * cache (padding).
  */
 CB_API int cb_gather_paged_kv4(const void* k_codes, const void* v_codes, int64_t block_stride,
                                int64_t slot_stride, int64_t head_stride, const void* k_scales,

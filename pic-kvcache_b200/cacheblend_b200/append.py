@@ -308,7 +308,8 @@ def gather_paged_kv4(
     """The values of 4-bit rows as ``[2, tokens, heads, head_size]`` of ``dtype``.
 
     A negative slot (padding) reads as zeros; so does, on the device, one outside the cache
-    (IndexError for host slots).
+    (IndexError for host slots).  A finite value past fp16's end (a step is rounded, so a group's highest
+    code may stand for up to 65,536) reads as +-65504 in fp16.
     """
     codes = cache.codes
     device = codes.get_device()

@@ -667,7 +667,8 @@ struct GatherParams {
   int units, units_block, tokens_block, threads;
 };
 
-// 16 values of HPT heads of K or V per thread; a slot outside the cache reads as zeros.
+// 16 values of HPT heads of K or V per thread; a slot outside the cache reads as zeros.  Values past fp16's
+// end are held there in fp16.
 template <typename T, bool WIDE, int HPT>
 __global__ void __launch_bounds__(kThreads) gather4_kernel(const GatherParams c) {
   const Place w = place<HPT>(c, c.heads, 0, c.head_size / 16);
@@ -702,6 +703,14 @@ __global__ void __launch_bounds__(kThreads) gather4_kernel(const GatherParams c)
         float y[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[j] = fmaf(static_cast<float>((word >> (4 * j)) & 15u), pair[i].x, pair[i].y);
+        if constexpr (std::is_same<T, __half>::value) {
+          // the step's rounding may take the highest code past fp16's end, which would read as an infinity
+          if (fabsf(pair[i].y) + 15.0f * fabsf(pair[i].x) > kHalfMax) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (fabsf(y[j]) < INFINITY) y[j] = fminf(fmaxf(y[j], -kHalfMax), kHalfMax);
+          }
+        }
         store_n<T, 8, WIDE>(row + 8 * s, y);
       }
     }

@@ -328,3 +328,19 @@ def test_4_bit_groups_at_the_ends_of_bf16(cuda, pad):
     want[2], want[2, 0, ::2] = 15 * 8736 - 65504, -65504  # a step of fp16(131008 / 15) = 8736
     got = gather_paged_kv4(cache, torch.arange(4, device=cuda), torch.float32)
     assert torch.equal(got[0], want) and torch.equal(got[1], want)
+
+
+def test_fp16_values_at_its_end_read_back_finite(cuda):
+    """A step is rounded, so a group's highest code may stand for more than fp16 holds: read at its end."""
+    x = torch.zeros(3, 1, 128, dtype=torch.float16, device=cuda)
+    x[0, 0, 5], x[1, 0, 70], x[2, 0, :64:2], x[2, 0, 1:64:2] = 65504.0, -65504.0, 65504.0, -65504.0
+    cache, at = PagedKV4.allocate(1, 3, 1, 128, cuda), torch.arange(3, device=cuda)
+    append_paged_kv4(None, None, x, x, cache, at)
+    wide = gather_paged_kv4(cache, at, torch.float32)
+    assert float(wide.max()) > 65504
+    for out in (None, torch.empty(2, 3, 1, 129, dtype=torch.float16, device=cuda)[..., 1:]):
+        got = gather_paged_kv4(cache, at, torch.float16, out=out)
+        assert torch.equal(got, wide.clamp(-65504, 65504).half())
+    cache.scales[0, 0, 0, 0, 0, 0], cache.scales[0, 0, 0, 1, 1, 1] = torch.nan, torch.inf  # what is not finite stays so
+    got = gather_paged_kv4(cache, at, torch.float16)
+    assert bool(got[0, 0, 0, :64].isnan().all()) and bool((got[0, 1, 0, 64:] == torch.inf).all())
