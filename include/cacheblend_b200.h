@@ -509,7 +509,7 @@ CB_API int cb_gather_paged_kv4(const void* k_codes, const void* v_codes, int64_t
  * and pages outside the cache are left out; a row that sees no key is zeros;
  * rows of no sequence are not written; query_start is clamped to the rows there
  * are.  Logits, softmax and sums in fp32, the weighted steps of the values
- * rounded to fp16 before the product with their codes.  `workspace`: 32-byte
+ * rounded to fp16 before the product with their codes.  scale: finite.  `workspace`: 32-byte
  * aligned device memory of cb_paged_attention4_workspace_size bytes, any
  * contents; calls that share one must not overlap on the GPU.
  */
@@ -537,7 +537,7 @@ CB_API int cb_paged_attention4(const void* query, int64_t query_token_stride,
  * sees the keys at or before k - n + j.  query, out: [num_queries][num_q_heads]
  * [head_size], key, value: [num_keys][num_kv_heads][head_size], bf16 or fp16,
  * heads of 64 or 128 values, at most 128 query heads to a KV head, token and
- * head strides in bytes, rows 16-byte aligned; scale > 0.  Logits, softmax and
+ * head strides in bytes, rows 16-byte aligned; scale > 0, finite.  Logits, softmax and
  * sums in fp32, the probabilities rounded to the element type for the second
  * product.  A query that sees no key gives zeros; rows of no sequence are not
  * written; starts are clamped to the rows there are.  What a masked place holds

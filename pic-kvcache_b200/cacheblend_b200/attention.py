@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 
 import torch
 
@@ -102,6 +103,7 @@ def blend_attention(
 
 
 _HALVES = (torch.bfloat16, torch.float16)
+_MOST = torch.finfo(torch.float32).max * math.log(2)  # a scale goes to fp32, and there to powers of two
 
 
 def _int32(name: str, tensor: torch.Tensor, device: int, ndim: int) -> None:
@@ -163,7 +165,7 @@ def paged_attention4(
 
     A row that sees no key (an empty sequence) is zeros; rows behind the last sequence are left
     as ``out`` held them.  Pages outside the cache and keys past the table's width are left
-    out.  ``workspace``: ``paged_attention4_workspace_bytes`` of uint8, for callers that keep one
+    out.  ``scale`` must be finite.  ``workspace``: ``paged_attention4_workspace_bytes`` of uint8, for callers that keep one
     (two calls that may overlap need two); otherwise allocated per call.
     """
     if query.ndim != 3:
@@ -193,6 +195,8 @@ def paged_attention4(
         start = query_start.data_ptr()
     elif tokens != seqs:
         raise ValueError(f"{tokens} query tokens for {seqs} sequences need query_start")
+    if not -_MOST < scale < _MOST:
+        raise ValueError(f"the scale must be finite, not {scale}")
     if device < 0:
         _native.require_cuda(query)
     with on_device(device, stream):
@@ -245,7 +249,7 @@ def prompt_attention(
 
     A query that sees no key gives zeros; rows of no sequence are left as ``out`` held them, and
     nothing that a masked place or another sequence holds reaches an output.  ``scale`` must be
-    positive.  ``workspace``: ``prompt_attention_workspace_bytes`` of uint8, for callers that keep
+    positive and finite.  ``workspace``: ``prompt_attention_workspace_bytes`` of uint8, for callers that keep
     one (two calls that may overlap need two); otherwise allocated per call.
     """
     shape, key_shape = query.shape, key.shape
@@ -277,8 +281,8 @@ def prompt_attention(
         _int32("key_start", key_start, device, 1)
         if key_start.numel() != seqs + 1:
             raise ValueError("key_start must hold as many entries as query_start")
-    if not scale > 0:
-        raise ValueError(f"the scale must be positive, not {scale}")
+    if not 0 < scale < _MOST:
+        raise ValueError(f"the scale must be positive and finite, not {scale}")
     if device_error is not None and (device_error.dtype != torch.int32 or device_error.get_device() != device):
         raise ValueError("device_error must be int32 on the query's device")
     if device < 0:

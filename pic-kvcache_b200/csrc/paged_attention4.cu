@@ -58,6 +58,7 @@
 // 55 % of the issue slots and 46 % of the ALU pipe with 16 warps an SM, beside some
 // 10 us of launch, first loads and the join.  The memory side alone takes 33 us.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "cb_common.cuh"
@@ -879,6 +880,7 @@ extern "C" int cb_paged_attention4(const void* query, int64_t query_token_stride
   CB_SUPPORTED(dtype == CB_DTYPE_BF16 || dtype == CB_DTYPE_FP16, "queries must be bf16 or fp16");
   const int rc = att4::check_shape(num_tokens, num_seqs, num_q_heads, num_kv_heads, head_size);
   if (rc != CB_OK) return rc;
+  CB_REQUIRE(std::isfinite(scale * att4::kLog2e), "the scale must be finite (got %g)", static_cast<double>(scale));
   if (num_tokens == 0) return CB_OK;
   CB_REQUIRE(query_start != nullptr || num_tokens == num_seqs, "one token per sequence, or query_start");
   CB_REQUIRE(num_blocks >= 0 && num_blocks < (int64_t(1) << 31) && block_size > 0 && block_size < (int64_t(1) << 22) &&

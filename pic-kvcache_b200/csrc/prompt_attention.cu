@@ -52,6 +52,7 @@
 // masked tiles and rolled loops in the epilogue took 9 prompts of 8,500 tokens from
 // 152 to 144 us.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "cb_common.cuh"
@@ -939,7 +940,8 @@ extern "C" int cb_prompt_attention(const void* query, int64_t query_token_stride
   int rc = prompt::check_shape(num_queries, num_seqs, num_q_heads, num_kv_heads, head_size);
   if (rc != CB_OK) return rc;
   CB_REQUIRE(num_keys >= 0 && num_keys < (int64_t(1) << 30), "size out of range");
-  CB_REQUIRE(scale > 0.0f, "the scale must be positive (got %g)", static_cast<double>(scale));
+  CB_REQUIRE(scale > 0.0f && std::isfinite(scale * prompt::kLog2e), "the scale must be positive and finite (got %g)",
+             static_cast<double>(scale));
   if (num_queries == 0 || num_seqs == 0) return CB_OK;
   CB_REQUIRE(query && query_start && key_start && out && workspace, "null pointer argument");
   CB_REQUIRE(num_keys == 0 || (key && value), "null key or value pointer");

@@ -122,3 +122,19 @@ def test_packed_calls_refuse_alike():
     values[14] = 1 << 32  # the element type's code is an int
     assert lib.cb_call_packed(code, 0, pack(*values), count) == _native.CB_ERR_INVALID
     assert b"fit" in lib.cb_last_error()
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 1e39])
+def test_scales_that_are_not_finite(scale):
+    """A scale that fp32 does not hold is refused, not taken for another."""
+    with pytest.raises(ValueError, match="scale"):
+        paged_attention4(Q, CACHE, TABLE, LENS, scale)
+    with pytest.raises(ValueError, match="scale"):
+        prompt_attention(Q, K, K, START, scale)
+    lib = _native.load_library()
+    assert lib.cb_paged_attention4(None, 0, 0, 2, 8, 0, None, None, None, 0, 0, 0, None, None, 0, 0, 0, 4, 16, 2, 128, None, 0, 0,
+                                   None, 2, scale, None, 0, 0, None, 0, None) == _native.CB_ERR_INVALID
+    assert b"scale" in lib.cb_last_error()
+    assert lib.cb_prompt_attention(None, 0, 0, None, 0, 0, None, 0, 0, 2, 2, 8, 2, 128, 0, None, None, 1, scale, None, 0, 0, None,
+                                   0, None, None) == _native.CB_ERR_INVALID
+    assert b"scale" in lib.cb_last_error()
