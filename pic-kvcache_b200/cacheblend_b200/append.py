@@ -180,7 +180,9 @@ def _rotation(rotary_emb, head_size: int, dtype: torch.dtype, device: int) -> tu
     """(table or None, table dtype code, positions it holds, rotary_dim, neox)."""
     if rotary_emb is None:
         return None, _native.DTYPE_CODES[torch.float32], 0, 0, 1
-    table = rotary_emb.cos_sin_cache
+    table = getattr(rotary_emb, "cos_sin_cache", None)
+    if table is None:
+        raise NotImplementedError("the append needs a rotary module with cos_sin_cache")
     rotary_dim = int(getattr(rotary_emb, "rotary_dim", head_size))
     if rotary_emb.head_size != head_size:
         raise ValueError(f"the rotation is made for heads of {rotary_emb.head_size} values, not {head_size}")

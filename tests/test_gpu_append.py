@@ -344,3 +344,14 @@ def test_fp16_values_at_its_end_read_back_finite(cuda):
     cache.scales[0, 0, 0, 0, 0, 0], cache.scales[0, 0, 0, 1, 1, 1] = torch.nan, torch.inf  # what is not finite stays so
     got = gather_paged_kv4(cache, at, torch.float16)
     assert bool(got[0, 0, 0, :64].isnan().all()) and bool((got[0, 1, 0, 64:] == torch.inf).all())
+
+
+def test_rotary_modules_without_a_table_are_refused(cuda):
+    bare = SimpleNamespace(head_size=64, rotary_dim=64, is_neox_style=True)
+    _, k, v, positions = _inputs(cuda, 3, 1, 2, 64, torch.bfloat16, 15)
+    pages, slots = torch.zeros(2, 4, 16, 2, 64, dtype=torch.bfloat16, device=cuda), torch.arange(3, device=cuda)
+    with pytest.raises(NotImplementedError, match="cos_sin_cache"):
+        append_paged_kv(bare, positions, k, v, pages, slots, 16)
+    with pytest.raises(NotImplementedError, match="cos_sin_cache"):
+        append_paged_kv4(bare, positions, k, v, PagedKV4.allocate(4, 16, 2, 64, cuda), slots)
+    assert int((pages != 0).sum()) == 0
