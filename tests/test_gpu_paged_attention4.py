@@ -389,3 +389,59 @@ def test_logits_past_fp32(cuda, size, sign):
     got = paged_attention4(query[:3], cache, table[:1], torch.tensor([2], dtype=torch.int32, device=cuda), 1.0,
                            query_start=torch.tensor([0, 3], dtype=torch.int32, device=cuda))
     assert int((got[0] != 0).sum()) == 0 and bool((got[1:] != 0).any(-1).all())
+
+
+@pytest.mark.parametrize("lens,block", [([40000], 128), ([9000, 300, 7001], 24)])
+@pytest.mark.parametrize("head", [64, 128])
+def test_every_part_counts(cuda, lens, block, head):
+    """Uniform weights and values that are zero but in one stretch of 256 keys (a CTA's round), swept over
+    the sequence: a part of a cut piece that is lost, or joined twice, changes an output by all of it.
+
+    Logits are 0, so exp2 and M are the same for every key.  A value is 15 steps of 1/8 over a lowest value
+    of 0: its factor is rounded to fp16 (2^-11) and weighs with 15 - 8 and, in fp32, 8; sums of up to
+    40,000 terms in fp32, in parts of at most some hundred a lane and then by tree: 2^-14.  The result is
+    rounded once."""
+    cache, table = _pages(cuda, lens, block, 2, head, 18, step=(0.0, 0.0), low=(0.0, 0.0))
+    cache.codes[1] = 255
+    query = torch.randn(len(lens), 8, head, device=cuda, generator=torch.Generator(device=cuda).manual_seed(1)).to(torch.float16)
+    lengths = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    got, want = [], []
+    for first in range(0, max(lens), 256):
+        marked = PagedKV4(cache.codes, cache.scales.clone())
+        counts = []
+        for i, n in enumerate(lens):
+            keys = torch.arange(min(first, n), min(first + 256, n), device=cuda)
+            marked.scales[1, table[i].long()[keys // block], :, keys % block, :, 0] = 0.125
+            counts.append(1.875 * len(keys) / n)
+        got.append(paged_attention4(query, marked, table, lengths, head ** -0.5))
+        want.append(counts)
+    want = torch.tensor(want, dtype=torch.float64, device=cuda)[..., None, None]
+    off = (torch.stack(got).double() - want).abs()
+    u = torch.finfo(torch.float16).eps / 2
+    assert bool((off <= want * (u + 2.0 ** -11 + 2.0 ** -14) + 2.0 ** -24).all())
+
+
+@pytest.mark.parametrize("key", [0, 255, 256, 511, 512, 8191, 16384, 20000, 32767, 39999])
+def test_one_key_takes_all(cuda, key):
+    """One key of 40,000 whose logit is far over the rest, anywhere: the output is its value."""
+    cache, table = _pages(cuda, [40000], 128, 2, 128, 19)
+    query = torch.ones(1, 16, 128, device=cuda, dtype=torch.bfloat16)
+    cache.scales[0, table[0, key // 128], :, key % 128] = 4.0  # values of 4 to 64, the others' -2.7 to 4.1
+    got = paged_attention4(query, cache, table, torch.tensor([40000], dtype=torch.int32, device=cuda), 0.25)
+    vv, vl = _parts(cache, table[0], 40000, 1)
+    want, mass = (vv + vl)[key].repeat_interleave(8, 0), (vv + vl.abs())[key].repeat_interleave(8, 0)
+    # its logit is some 1,000 over the others': p is 1 and 0, one factor rounded to fp16, and the result
+    u = torch.finfo(query.dtype).eps / 2
+    assert bool(((got[0].double() - want).abs() <= u * want.abs() + (2.0 ** -11 + 2.0 ** -20) * mass).all())
+
+
+@pytest.mark.parametrize("case", CASES, ids=str)
+def test_outputs_are_finite(cuda, case):
+    """_check takes a maximum, which passes over NaN: whatever the pages hold behind a sequence's end, none comes out."""
+    lens, block, heads, kv_heads, head, dtype, counts = case
+    cache, table = _pages(cuda, lens, block, kv_heads, head, 3)
+    total = len(lens) if counts is None else sum(counts)
+    query = torch.randn(total, heads, head, generator=torch.Generator(device=cuda).manual_seed(4), device=cuda).to(dtype)
+    begin = None if counts is None else torch.tensor([0, *torch.tensor(counts).cumsum(0).tolist()], dtype=torch.int32, device=cuda)
+    got = paged_attention4(query, cache, table, torch.tensor(lens, dtype=torch.int32, device=cuda), head ** -0.5, query_start=begin)
+    assert bool(got.isfinite().all())
