@@ -325,3 +325,54 @@ def test_no_keys_at_all(cuda):
         got = prompt_attention(q, k, v, starts, 0.125, key_start=torch.zeros_like(starts), out=out)
         end = 2 + sum(lengths)
         assert int((got[2:end] != 0).sum()) == 0 and bool((got[:2] == 3).all()) and bool((got[end:] == 3).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("queries,keys,head", [(1, 5001, 128), (5, 5001, 64), (200, 5001, 128)])
+def test_every_tile_counts(cuda, dtype, queries, keys, head):
+    """Uniform weights, and per KV head values that are 1 in one tile of 128 keys and 0 elsewhere: a tile
+    that is lost or taken twice changes an output by all of it.
+
+    Logits are 0 and probabilities a power of two, so the sums are exact (up to 5,001 ones); the quotient
+    is off by 2 ulp of fp32 and the result is rounded once."""
+    tiles = -(-keys // 128)
+    q, k, v = _inputs(cuda, queries, keys, tiles, tiles, head, dtype, 15)
+    k.zero_()
+    at = torch.arange(keys, device=cuda)
+    v[:] = (at[:, None] // 128 == torch.arange(tiles, device=cuda)).to(dtype)[..., None]
+    got = prompt_attention(q, k, v, _starts([queries], cuda), head ** -0.5, key_start=_starts([keys], cuda))
+    seen = keys - queries + 1 + torch.arange(queries, device=cuda)[:, None]
+    count = (seen - torch.arange(tiles, device=cuda) * 128).clamp(0, 128)
+    want = (count.double() / seen)[..., None]
+    assert bool(((got.double() - want).abs() <= want * (torch.finfo(dtype).eps / 2 + 2.0 ** -20)).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_one_key_of_a_long_prefix_takes_all(cuda, dtype):
+    """Per KV head one key far over the rest, in the first tile, the last and each between.
+
+    fp16: the probabilities' subnormals are off by n 2^-32 max |v| (see above)."""
+    keys, head, kv_heads = 5001, 128, 40
+    q, k, v = _inputs(cuda, 3, keys, kv_heads, kv_heads, head, dtype, 16)
+    planted = torch.arange(kv_heads, device=cuda) * 128 + torch.arange(kv_heads, device=cuda) * 37 % 128
+    planted = planted.clamp(max=keys - 3)
+    heads = torch.arange(kv_heads, device=cuda)
+    q[:] = q[:1]
+    k[planted, heads] = q[0]  # a logit of |q|^2 / 4, about 32, against +-2.8
+    got = prompt_attention(q, k, v, _starts([3], cuda), 0.25, key_start=_starts([keys], cuda))
+    want, bound = _want(q, k, v, 0.25)
+    if dtype == torch.float16:
+        bound -= keys * (2.0 ** -17 - 2.0 ** -32) * v.double().abs().amax((0, 2))[:, None]
+    bound += want.abs() * (torch.finfo(dtype).eps / 2) + 2.0 ** -24
+    assert float(((got.double() - want).abs() / bound).max()) <= 1
+    assert float((want - v[planted, heads].double()).abs().max()) < 0.05  # the planted key's value it is
+
+
+@pytest.mark.parametrize("case", CASES, ids=lambda c: f"{len(c[0])}x{max(c[0])}-{c[2]}-{c[3]}-{c[4]}-{c[5]}"[:60])
+def test_outputs_are_finite(cuda, case):
+    """_check takes a maximum, which passes over NaN: no output is one."""
+    lengths, prefix, heads, kv_heads, head, dtype = case
+    key_lengths = lengths if prefix is None else [n + p for n, p in zip(lengths, prefix)]
+    q, k, v = _inputs(cuda, sum(lengths), sum(key_lengths), heads, kv_heads, head, dtype, 1)
+    got = prompt_attention(q, k, v, _starts(lengths, cuda), head ** -0.5, key_start=_starts(key_lengths, cuda))
+    assert bool(got.isfinite().all())
