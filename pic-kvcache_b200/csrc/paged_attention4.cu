@@ -15,9 +15,11 @@
 // memory first: 46 codes a clock and SM at the memory's rate are 92 bytes of its
 // 128, before any is read.  From registers a code costs under one instruction:
 //   * a masked word is two fp16 at once: a nibble at bits 0-3 of a half is the
-//     subnormal c 2^-24, at bits 4-7 c 2^-20, both exact in the tensor core.  The
-//     factor 2^24 goes into the row's factor, the odd nibbles' 16 into q (K) or
-//     into the output row (V).
+//     subnormal c 2^-24, at bits 4-7 c 2^-20, both exact operands.  The factor 2^24
+//     goes into the row's factor, the odd nibbles' 16 into q (K) or into the output row
+//     (V).  A product lines its terms up by the operands' exponents, a subnormal's being
+//     2^-14, so that its sum is cut at about 2^-14 of a factor (measured: 2^-18.6 of 8
+//     factors): coarser than fp32, but an eighth of what rounding the factor may cost.
 //   * K: the 16 keys of a tile are the M rows, the query rows the N columns, the
 //     dimensions of one group the K steps.  Eight columns: a whole group of query
 //     heads usually fits, and 16 at once, which share the masked words, ran with half

@@ -445,3 +445,52 @@ def test_outputs_are_finite(cuda, case):
     begin = None if counts is None else torch.tensor([0, *torch.tensor(counts).cumsum(0).tolist()], dtype=torch.int32, device=cuda)
     got = paged_attention4(query, cache, table, torch.tensor(lens, dtype=torch.int32, device=cuda), head ** -0.5, query_start=begin)
     assert bool(got.isfinite().all())
+
+
+def _centred_bound(q, step, varied, low, key_step, keys, p, scale, info):
+    """What one query head of 64 bits may be off by, whatever the steps and lowest values are.
+
+    With factors f_j = p_j step_j, codes c_j and middles m_j = low_j + 8 step_j:
+
+    * a factor is rounded to fp16 and weighs with c - 8: 2^-11 sum f |c - 8| (and the subnormals, see
+      test_rows_of_very_different_step);
+    * a product of the matrix unit lines its terms up by the fp16 exponents of the operands, and a code is a
+      subnormal 2^-24 c, whose exponent counts as 2^-14: sums are cut 2^10 above fp32's 2^-24 (measured:
+      2^-18.6 of 8 f), at most 2^-13 of each product's largest factor: 2^-13 sum f.  The same for the logits:
+      4 products a group cut at 2^-13 max |q| step, in log2 scale log2e; 2^-10 scale max |q| max step covers both
+      groups, twice (numerator and sum);
+    * fp32 logits, exp2 and sums: 2^-15 (A + 1) of sum p |m| + f |c - 8|, A = scale log2e sum |q| |k|;
+    * the result is rounded once."""
+    e = torch.einsum("hgl,lhd->hgd", p, (varied - 8 * step).abs())
+    everything = e + torch.einsum("hgl,lhd->hgd", p, (low + 8 * step).abs())
+    factors = torch.einsum("hgl,lhd->hgd", p, step)
+    largest = torch.einsum("hgl,lhd->hgld", p, step).amax((2, 3))[..., None]
+    size = torch.einsum("hgd,lhd->hgl", q.abs(), keys).amax(-1)[..., None] * abs(scale) * math.log2(math.e)
+    cut = 2.0 ** -9 * abs(scale) * q.abs().amax(-1)[..., None] * key_step
+    return 2.0 ** -11 * e + 2.0 ** -13 * factors + (2.0 ** -15 * (size + 1) + cut) * everything \
+        + len(step) * 2.0 ** -32 * largest + info.smallest_normal
+
+
+@pytest.mark.parametrize("step", [(1e-3, 5.0), (0.0, 0.01)])
+@pytest.mark.parametrize("low", [(-30.0, 10.0), (-0.1, 0.1)])
+@pytest.mark.parametrize("lens,block,heads,kv_heads,head,dtype", [
+    ([1, 20, 700, 3], 16, 16, 2, 128, torch.bfloat16), ([16, 1, 5, 2000], 24, 10, 5, 64, torch.float16),
+    ([9000], 128, 8, 8, 128, torch.float16), ([2] * 40, 33, 24, 8, 64, torch.bfloat16)])
+def test_wide_steps_and_lowest_values(cuda, lens, block, heads, kv_heads, head, dtype, step, low):
+    cache, table = _pages(cuda, lens, block, kv_heads, head, 22, step, low)
+    query = torch.randn(len(lens), heads, head, device=cuda, generator=torch.Generator(device=cuda).manual_seed(1)).to(dtype)
+    scale = head ** -0.5
+    got = paged_attention4(query, cache, table, torch.tensor(lens, dtype=torch.int32, device=cuda), scale)
+    info = torch.finfo(dtype)
+    key_step = float(cache.scales[0, ..., 0].nan_to_num(0).max())
+    for i, n in enumerate(lens):
+        kv, kl = _parts(cache, table[i], n, 0)
+        vv, vl = _parts(cache, table[i], n, 1)
+        pages = table[i, :-(-n // block)].long()
+        steps = cache.scales[1][pages][..., :1].double().expand(-1, -1, -1, -1, 64).flatten(-2).transpose(1, 2).flatten(0, 1)[:n]
+        q = query[i].double().unflatten(0, (kv_heads, -1))
+        p = torch.softmax(torch.einsum("hgd,lhd->hgl", q, kv + kl) * scale, -1)
+        want = torch.einsum("hgl,lhd->hgd", p, vv + vl)
+        bound = want.abs() * (info.eps / 2) + _centred_bound(q, steps, vv, vl, key_step, kv + kl.abs(), p, scale, info)
+        off = (got[i].double().unflatten(0, (kv_heads, -1)) - want).abs()
+        assert bool((off <= bound).all()), (i, float((off / bound).max()))
