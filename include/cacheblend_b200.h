@@ -485,8 +485,8 @@ CB_API int cb_append_paged_kv4(const void* key, int64_t key_token_stride, int64_
 
 /*
  * Rows of 4-bit pages as values: out[plane, t] = the row of slots[t], rounded
- * once to `dtype` (fp16: finite values past its end are held there); zeros for a slot outside the
- * cache (padding).
+ * once to `dtype` (fp16: finite values past its end are held there); zeros for a
+ * slot outside the cache (padding).
  */
 CB_API int cb_gather_paged_kv4(const void* k_codes, const void* v_codes, int64_t block_stride,
                                int64_t slot_stride, int64_t head_stride, const void* k_scales,
@@ -509,9 +509,11 @@ CB_API int cb_gather_paged_kv4(const void* k_codes, const void* v_codes, int64_t
  * and pages outside the cache are left out; a row that sees no key is zeros;
  * rows of no sequence are not written; query_start is clamped to the rows there
  * are.  Logits, softmax and sums in fp32, the weighted steps of the values
- * rounded to fp16 before the product with their codes.  scale: finite.  `workspace`: 32-byte
- * aligned device memory of cb_paged_attention4_workspace_size bytes, any
- * contents; calls that share one must not overlap on the GPU.
+ * rounded to fp16 before the product with their codes.  A V group whose step is
+ * not finite gives NaN in its own 64 dimensions.  scale: finite.  Page pointers
+ * may not be NULL, not even for num_blocks 0.  `workspace`: 32-byte aligned
+ * device memory of cb_paged_attention4_workspace_size bytes, any contents;
+ * calls that share one must not overlap on the GPU.
  */
 CB_API int cb_paged_attention4_workspace_size(int64_t num_tokens, int64_t num_seqs,
                                               int64_t num_q_heads, int64_t num_kv_heads,
@@ -537,11 +539,12 @@ CB_API int cb_paged_attention4(const void* query, int64_t query_token_stride,
  * sees the keys at or before k - n + j.  query, out: [num_queries][num_q_heads]
  * [head_size], key, value: [num_keys][num_kv_heads][head_size], bf16 or fp16,
  * heads of 64 or 128 values, at most 128 query heads to a KV head, token and
- * head strides in bytes, rows 16-byte aligned; scale > 0, finite.  Logits, softmax and
- * sums in fp32, the probabilities rounded to the element type for the second
- * product.  A query that sees no key gives zeros; rows of no sequence are not
- * written; starts are clamped to the rows there are.  What a masked place holds
- * (NaN, infinities) reaches no output.  `workspace`: 16-byte aligned device
+ * head strides in bytes, rows 16-byte aligned; scale > 0, finite.  Logits,
+ * softmax and sums in fp32, the probabilities rounded to the element type for
+ * the second product.  A query that sees no key gives zeros (num_keys 0: every
+ * one; key and value may then be NULL), one whose seen logits are all -inf NaN;
+ * rows of no sequence are not written; starts are clamped to the rows there
+ * are.  What a masked place holds (NaN, infinities) reaches no output.  `workspace`: 16-byte aligned device
  * memory of cb_prompt_attention_workspace_size bytes, any contents; calls that
  * share one must not overlap on the GPU.  On the tensor cores (tcgen05.mma, TMA);
  * device_error (optional) receives a code if a bounded wait gives up.

@@ -34,7 +34,8 @@ class PagedKV4:
     ``[2, num_blocks, num_heads, block_size, head_size // 64, 2]``, each group's step and
     lowest value: a value is ``lowest + step * code``.  Plane 0 is K, plane 1 V.  The rows
     of both are contiguous; the other strides are free (a view of a larger pool will do).
-    Head sizes 64 and 128.
+    Head sizes 64 and 128.  Steps and lowest values are finite, but for groups that are not: their
+    step is NaN, and whatever sees such a group of V has NaN in its 64 dimensions, of K in all.
     """
 
     codes: torch.Tensor
@@ -249,7 +250,8 @@ def append_paged_kv(
     ``query`` ``[tokens, q_heads, head_size]`` rotated at the same positions, in a new tensor,
     or None without one.
 
-    The products and their sum are rounded to fp32 each, and once to the element type.
+    The products and their sum are rounded to fp32 each, and once to the element type; a float32
+    table is used as it is (``relocate_key`` rounds it, and each product, to the keys' type).
     Slots and positions on the host are range-checked (IndexError); on the device a slot
     outside the cache, or a position outside the table, leaves the pages as they were (and
     gives a zero query row).

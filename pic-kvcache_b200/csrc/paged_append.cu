@@ -7,7 +7,8 @@
 //   GPT-J   the same with the partners 2i and 2i + 1
 // The table is read in its own type, both products and the sum are rounded to
 // fp32 one by one (no contraction), and the result is rounded once to the
-// element type: a cached row is the same bits whatever launch wrote it.
+// element type: a row is the same bits whichever of these kernels wrote it.  (The
+// relocation of cached keys rounds the table and every product to the key type.)
 //
 // 4-bit rows: every 64 values of a row share a lowest value and a step,
 //   low = fp16(min x), step = fp16((max x - low') / 15)   (low' = the fp32 minimum)
@@ -20,6 +21,8 @@
 //
 // What bounds them: HBM at long prompts, the launch at decode sizes.  Threads of
 // a block run over one token's pieces first, so rows are read and written whole.
+// Rows that are not 16-byte aligned go value by value: 16,384 tokens of 32 + 8 + 8
+// heads 700 us (67 aligned), 20,011 tokens into 4-bit pages 79 us (40).
 #include <algorithm>
 #include <type_traits>
 

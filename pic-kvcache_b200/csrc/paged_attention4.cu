@@ -56,9 +56,10 @@
 // launch joins them in order, so a result does not depend on timing.
 //
 // What bounds it (6 sequences of up to 98,304 keys, 32 query heads on 4: 40 us, 3.8
-// TB/s): about 500 instructions a tile, 160 of them the codes' masks and shifts, at
-// 55 % of the issue slots and 46 % of the ALU pipe with 16 warps an SM, beside some
-// 10 us of launch, first loads and the join.  The memory side alone takes 33 us.
+// TB/s, replayed from a graph; 41 to 51 us call by call): about 500 instructions a
+// tile, 160 of them the codes' masks and shifts, at 55 % of the issue slots and 46 % of
+// the ALU pipe with 16 warps an SM, beside some 10 us of launch, first loads and the
+// join.  The memory side alone takes 33 us.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
