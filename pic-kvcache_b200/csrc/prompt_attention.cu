@@ -45,8 +45,9 @@
 // *device_error, the CTA drains its MMAs and loads, frees TMEM and returns.
 //
 // What bounds it (16,384 tokens, 32 heads on 8, D 128: 1,635 us, 1,345 TFLOP/s; 1,850 to
-// 1,900 once the power cap holds the clocks): the chain S, P, P V, S of one tile, 2,880 cycles even where it runs alone, in a pair's
-// period of 3,150; the tensor cores and the MUFU (16 exp2 a clock) need 2,048 each.
+// 1,900 us once the power cap holds the clocks): the chain S, P, P V, S of one tile, 2,880
+// cycles even where it runs alone, in a pair's period of 3,150; the tensor cores and the
+// MUFU (16 exp2 a clock) need 2,048 each.
 // The softmax warps' code is kept short: what runs once per item is fetched anew each
 // time (about 4 cycles an instruction).  One copy of the tile's code for whole and
 // masked tiles and rolled loops in the epilogue took 9 prompts of 8,500 tokens from
