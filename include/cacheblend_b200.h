@@ -544,9 +544,10 @@ CB_API int cb_paged_attention4(const void* query, int64_t query_token_stride,
  * the second product.  A query that sees no key gives zeros (num_keys 0: every
  * one; key and value may then be NULL), one whose seen logits are all -inf NaN;
  * rows of no sequence are not written; starts are clamped to the rows there
- * are.  What a masked place holds (NaN, infinities) reaches no output.  `workspace`: 16-byte aligned device
- * memory of cb_prompt_attention_workspace_size bytes, any contents; calls that
- * share one must not overlap on the GPU.  On the tensor cores (tcgen05.mma, TMA);
+ * are.  What a masked place holds (NaN, infinities) reaches no output.
+ * `workspace`: 16-byte aligned device memory of
+ * cb_prompt_attention_workspace_size bytes, any contents; calls that share one
+ * must not overlap on the GPU.  On the tensor cores (tcgen05.mma, TMA);
  * device_error (optional) receives a code if a bounded wait gives up.
  */
 CB_API int cb_prompt_attention_workspace_size(int64_t num_queries, int64_t num_seqs,

@@ -164,9 +164,10 @@ def paged_attention4(
     ``seq_lens - n + j``.
 
     A row that sees no key (an empty sequence) is zeros; rows behind the last sequence are left
-    as ``out`` held them.  Pages outside the cache and keys past the table's width are left
-    out; a cache of no pages is refused.  Logits are fp32: a row whose logits it does not hold or tell
-    apart (beyond 2^30 or so) need not come out finite.  ``scale`` must be finite.  ``workspace``: ``paged_attention4_workspace_bytes`` of uint8, for callers that keep one
+    as ``out`` held them.  Pages outside the cache and keys past the table's width are left out;
+    a cache of no pages is refused.  Logits are fp32: a row whose logits it does not hold or tell
+    apart (beyond 2^30 or so) need not come out finite.  ``scale`` must be finite.
+    ``workspace``: ``paged_attention4_workspace_bytes`` of uint8, for callers that keep one
     (two calls that may overlap need two); otherwise allocated per call.
     """
     if query.ndim != 3:
@@ -253,7 +254,8 @@ def prompt_attention(
     logits are all -inf is NaN, as of any softmax of them.  Probabilities are rounded to the
     element type before they meet the values.  ``scale`` must be positive and finite.
     ``device_error``: int32, set to a code if a wait inside the kernel ran out of its 2 seconds
-    (rows are then missing); without it that goes unreported.  ``workspace``: ``prompt_attention_workspace_bytes`` of uint8, for callers that keep
+    (rows are then missing); without it that goes unreported.
+    ``workspace``: ``prompt_attention_workspace_bytes`` of uint8, for callers that keep
     one (two calls that may overlap need two); otherwise allocated per call.
     """
     shape, key_shape = query.shape, key.shape
